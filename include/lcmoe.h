@@ -48,10 +48,13 @@ typedef enum {
 /* GGUF ggml_type codes, QuantType::code, rust/src/model/quant.rs:45-73. */
 enum {
     LCMOE_TYPE_F32 = 0,
+    LCMOE_TYPE_F16 = 1,  /* activations, logits and K/V caches only        */
     LCMOE_TYPE_Q4_0 = 2, /* lcmoe_shard_matmul only: the shard engine's Q4_0 */
     LCMOE_TYPE_Q8_0 = 8,
     LCMOE_TYPE_Q4_K = 12,
-    LCMOE_TYPE_Q6_K = 14
+    LCMOE_TYPE_Q6_K = 14,
+    LCMOE_TYPE_I8 = 24,  /* K/V caches only                                */
+    LCMOE_TYPE_BF16 = 30 /* activations and logits only                    */
 };
 
 /* Router kinds.  The reference has no router; these are the written
@@ -472,6 +475,135 @@ lcmoe_status lcmoe_matmul_f32(const float *a, const float *b, float *c, int32_t 
  * stream); returns without waiting. */
 lcmoe_status lcmoe_matmul_f32_dev(const float *a_dev, const float *b_dev, float *c_dev, int32_t m,
                                   int32_t k, int32_t n, void *stream);
+
+/* ---- paged K/V cache and its attention -------------------------------- */
+
+/* A cache of keys and values in pages of page_tokens tokens, which sequences
+ * take from one pool through a page table: the reference's KVCache
+ * (rust/src/cache/mod.rs:18-126) for serving many sequences of unlike lengths,
+ * in f16 as there or in 8 bits.  All calls take device buffers, enqueue on
+ * `stream` (NULL: the null stream), allocate nothing and do not wait; they may
+ * be captured into a HIP graph.  Buffers live on the stream's device.
+ *
+ * 8 bits (LCMOE_TYPE_I8): a value is code * scale, code in [-127, 127], one
+ * f32 scale per page, K/V head and keys or values.  A page's scale is the
+ * largest magnitude appended to it / 127, so it grows as tokens come: the
+ * codes that are there are then rounded again to the new scale, by at most
+ * half a step each time. */
+typedef struct {
+    int32_t n_head, n_kv_head; /* query heads, a multiple of the K/V heads  */
+    int32_t head_dim;          /* a multiple of 16 in [16, 256]             */
+    int32_t page_tokens;       /* 16, 32, 64, 128 or 256                    */
+    int32_t n_pages;           /* pages of the pool                         */
+    int32_t max_pages;         /* pages of a sequence: the page table's row */
+    int32_t kv_type;           /* LCMOE_TYPE_F16 or LCMOE_TYPE_I8           */
+    int32_t act_type;          /* of k, v, q and results: LCMOE_TYPE_F32,
+                                  _F16 or _BF16                             */
+    int32_t rope_positions;    /* LCMOE_ROPE_*, where a call takes `rope`   */
+} lcmoe_kv_desc;
+
+/* The pool, on the device: k and v of lcmoe_kv_sizes' pool_bytes each, 16-byte
+ * aligned; scale [n_pages][n_kv_head][2] f32 (I8 only; keys, values), 8-byte
+ * aligned.  Need not be cleared.  A page holds, per K/V head, units of 16
+ * tokens in the order the attention's matrix instructions take them; read it
+ * with lcmoe_kv_read_dev. */
+typedef struct {
+    void *k, *v;
+    float *scale;
+} lcmoe_kv_pool;
+
+/* A ragged batch, its arrays on the device.  Sequence b has lens[b] tokens in
+ * the cache before the call and takes rows starts[b] .. starts[b + 1] - 1 of
+ * the call's operands as its next tokens (none: no rows); token i of them has
+ * position lens[b] + i.  starts is [n_seq + 1], from 0, never falling; NULL
+ * means max_new rows for every sequence (n_rows = n_seq * max_new).  max_new
+ * is at least the most rows of any sequence and n_rows at least
+ * starts[n_seq]; they size the launches, and rows past starts[n_seq] are left
+ * as they are.  pages [n_seq][max_pages]: page p of sequence b holds its
+ * positions p * page_tokens on; an id outside [0, n_pages) is a page that is
+ * not there (nothing is written to it, its keys are not attended to, it reads
+ * as zeros).  Tokens at positions past max_pages * page_tokens are dropped,
+ * and their rows left as they are.  Sequences may share pages that no call
+ * appends to. */
+typedef struct {
+    int32_t n_seq, n_rows, max_new;
+    const int32_t *starts, *lens, *pages;
+} lcmoe_kv_batch;
+
+/* Bytes of k (and of v) and of scale (0 for F16).  Needs no GPU. */
+lcmoe_status lcmoe_kv_sizes(const lcmoe_kv_desc *desc, size_t *pool_bytes, size_t *scale_bytes);
+
+/* out [n_pos][head_dim / 2][2] (host): cosine and sine of p * theta^(-2 i /
+ * head_dim), computed in 64 bits and rounded once; apply_rotary_emb's angles
+ * (rust/src/inference/attention.rs:13-34), which keep their accuracy at far
+ * positions.  Needs no GPU. */
+lcmoe_status lcmoe_rope_table(float theta, int32_t head_dim, int32_t n_pos, float *out);
+
+/* Appends the batch's keys and values (rows of n_kv_head * head_dim, ld_k and
+ * ld_v elements apart; they may lie in one projection's rows).  rope
+ * [max_pages * page_tokens][head_dim / 2][2] as lcmoe_rope_table lays it out,
+ * on the device, 8-byte aligned: key dims d and d + head_dim / 2 are rotated
+ * (y_d = x_d cos - x_h sin, y_h = x_d sin + x_h cos) by the token's position
+ * (LCMOE_ROPE_ABSOLUTE) or its number in the call (PER_CALL); NULL: keys are
+ * stored as they are.  Rotation and quantisation run in 64 bits, so that a
+ * code is the exact value's.  F16: rounded once.  I8: infinities become the
+ * ends of the scale that the finite values have, NaN becomes 0.  Replaces
+ * KVCache::append (cache/mod.rs:33-63) and the keys' apply_rotary_emb. */
+lcmoe_status lcmoe_kv_append_dev(const lcmoe_kv_desc *desc, const lcmoe_kv_pool *pool,
+                                 const lcmoe_kv_batch *batch, const void *k_dev, int64_t ld_k,
+                                 const void *v_dev, int64_t ld_v, const float *rope_dev,
+                                 void *stream);
+
+/* KVCache::get (cache/mod.rs:65-78): the values that the cache holds at the
+ * batch's positions lens[b] + i, as rows of k and v. */
+lcmoe_status lcmoe_kv_read_dev(const lcmoe_kv_desc *desc, const lcmoe_kv_pool *pool,
+                               const lcmoe_kv_batch *batch, void *k_dev, int64_t ld_k, void *v_dev,
+                               int64_t ld_v, void *stream);
+
+/* out = softmax(scale * q k^T) v for the batch's rows, query head h on K/V
+ * head h / (n_head / n_kv_head), over the positions up to the row's own
+ * (attention_forward's core, attention.rs:56-115), which lcmoe_kv_append_dev
+ * has put there.  q and out: rows of n_head * head_dim, not overlapping.
+ * rope: as for the append, q is rotated on the way; NULL: q is taken as it
+ * is.  Scores, softmax and sums in f32; an f32 q and its probabilities enter
+ * the products as two f16 each, f16 and bf16 ones as one.  A row with nothing
+ * to attend to (every page missing) is zeros.  workspace: at least
+ * lcmoe_kv_attention_workspace's bytes, 16-byte aligned; its contents do not
+ * matter, and calls that may overlap in time (two streams, two graphs) need
+ * one each.  The workspace depends on desc and on the batch's three counts. */
+lcmoe_status lcmoe_kv_attention_workspace(const lcmoe_kv_desc *desc, const lcmoe_kv_batch *batch,
+                                          size_t *bytes);
+lcmoe_status lcmoe_kv_attention_dev(const lcmoe_kv_desc *desc, const lcmoe_kv_pool *pool,
+                                    const lcmoe_kv_batch *batch, const void *q_dev, int64_t ld_q,
+                                    const float *rope_dev, float scale, void *out_dev,
+                                    int64_t ld_out, void *workspace, size_t workspace_bytes,
+                                    void *stream);
+
+/* ---- log probabilities ------------------------------------------------ */
+
+/* For each row of logits [n_rows][vocab] (rows ld elements apart; F32, F16 or
+ * BF16): given_lp [n_rows][n_given] = log softmax at the token ids given
+ * [n_rows][n_given] (0 for an id outside [0, vocab): it adds nothing to a
+ * sum); entropy [n_rows] in nats (NULL: not wanted); the n_top (at most
+ * LCMOE_LOGPROBS_TOP) largest logits' ids and log probabilities, largest
+ * first, the lower id first among equals (NaN ranks as -inf; id -1 and -inf
+ * past the vocabulary).  Logits of -inf have no probability; a row of
+ * nothing else gives -inf and entropy 0, one with NaN or +inf gives NaN.
+ * Sums in f32.  The reference samples from these probabilities
+ * (rust/src/inference/sampler.rs:6-50) and does not report them.
+ * Device buffers, stream and workspace as in lcmoe_kv_attention_dev. */
+#define LCMOE_LOGPROBS_TOP 32
+lcmoe_status lcmoe_logprobs_workspace(int32_t type, int32_t n_rows, int32_t vocab, int32_t n_given,
+                                      int32_t n_top, size_t *bytes);
+lcmoe_status lcmoe_logprobs_dev(int32_t type, const void *logits_dev, int64_t ld, int32_t n_rows,
+                                int32_t vocab, const int32_t *given_dev, int32_t n_given,
+                                float *given_lp_dev, float *entropy_dev, int32_t n_top,
+                                int32_t *top_id_dev, float *top_lp_dev, void *workspace,
+                                size_t workspace_bytes, void *stream);
+/* Host buffers, synchronous. */
+lcmoe_status lcmoe_logprobs(int32_t type, const void *logits, int64_t ld, int32_t n_rows,
+                            int32_t vocab, const int32_t *given, int32_t n_given, float *given_lp,
+                            float *entropy, int32_t n_top, int32_t *top_id, float *top_lp);
 
 /* ---- device self-tests (need a GPU; used by the parity tests) ---------- */
 

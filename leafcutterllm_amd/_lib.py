@@ -15,6 +15,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("LCMOE_LIB") or os.path.join(_HERE, "liblcmoe.so")
 
 TYPE_F32, TYPE_Q8_0, TYPE_Q4_K, TYPE_Q6_K = 0, 8, 12, 14
+TYPE_F16, TYPE_I8, TYPE_BF16 = 1, 24, 30  # activations, logits and K/V caches only
 TYPE_Q4_0 = 2  # lcmoe_shard_matmul only: the shard engine's interleaved Q4_0
 ROUTE_SOFTMAX_RENORM, ROUTE_SOFTMAX, ROUTE_SIGMOID_GROUP = 0, 1, 2
 ACT_F16, ACT_F16X2 = 0, 1  # lcmoe_set_act_precision
@@ -41,7 +42,10 @@ EXPORTS = (
     "lcmoe_model_last_timing", "lcmoe_model_set_decode_graph", "lcmoe_matmul_f32",
     "lcmoe_matmul_f32_dev", "lcmoe_debug_route_fallbacks", "lcmoe_debug_read_bandwidth",
     "lcmoe_dequantize", "lcmoe_sanitize_blocks", "lcmoe_model_debug_fail_forward",
-    "lcmoe_model_debug_layer_moe", "lcmoe_set_act_precision",
+    "lcmoe_model_debug_layer_moe", "lcmoe_set_act_precision", "lcmoe_kv_sizes",
+    "lcmoe_rope_table", "lcmoe_kv_append_dev", "lcmoe_kv_read_dev",
+    "lcmoe_kv_attention_workspace", "lcmoe_kv_attention_dev", "lcmoe_logprobs_workspace",
+    "lcmoe_logprobs_dev", "lcmoe_logprobs",
 )
 
 

@@ -244,6 +244,34 @@ hipError_t launch_advance(int32_t *lens, int seq0, int nseq, int T, int32_t *ste
                           hipStream_t st);
 int64_t attention_part_floats(int nq, int H, int hd, int ctx);
 
+// ---- paged K/V cache (kv_device.h has its layout) and log probabilities ----
+
+// A cache pool and a call's ragged batch, checked by the C entry points
+// (include/lcmoe.h: lcmoe_kv_desc, lcmoe_kv_pool, lcmoe_kv_batch).
+struct KvArgs {
+    uint8_t *k, *v;
+    float *scale;  // [n_pages][KVH][2] (keys, values); 8 bits only
+    const int32_t *starts, *lens, *pages;
+    int n_seq, n_rows, max_new;
+    int H, KVH, hd, hdp;  // hdp: head_dim rounded up to 32
+    int plog;             // log2 of the tokens per page
+    int n_pages, max_pages, rope_abs, act;
+    bool i8;
+};
+// vec: rows start on 16 bytes and are whole 16-byte groups apart
+hipError_t launch_kv_append(const KvArgs &a, const void *k, int64_t ldk, const void *v, int64_t ldv,
+                            const float *rope, bool vec, hipStream_t st);
+hipError_t launch_kv_read(const KvArgs &a, void *k, int64_t ldk, void *v, int64_t ldv, bool vec,
+                          hipStream_t st);
+int64_t kv_attention_floats(const KvArgs &a);
+hipError_t launch_kv_attention(const KvArgs &a, const void *q, int64_t ldq, const float *rope,
+                               float scale, void *out, int64_t ldo, bool vec, float *ws,
+                               hipStream_t st);
+int64_t logprobs_bytes(int type, int rows, int vocab, int top);
+hipError_t launch_logprobs(int type, const void *x, int64_t ld, int rows, int vocab,
+                           const int32_t *given, int n_given, float *given_lp, float *entropy,
+                           int top, int32_t *top_id, float *top_lp, void *ws, hipStream_t st);
+
 hipError_t launch_debug_dequant(int qt, const uint8_t *src, int64_t count, float *out,
                                 hipStream_t st);
 hipError_t launch_debug_sigmoid(const float *x, int64_t n, float *out, hipStream_t st);

@@ -425,6 +425,24 @@ extern "C" lcmoe_status lcmoe_quantize(int32_t type, const float *src, uint8_t *
     return LCMOE_OK;
 }
 
+extern "C" lcmoe_status lcmoe_rope_table(float theta, int32_t head_dim, int32_t n_pos, float *out) {
+    clear_error();
+    if (!(theta > 0.0f) || !std::isfinite(theta))
+        return fail(LCMOE_ERR_INVALID_ARG, "theta must be finite and > 0");
+    if (head_dim < 2 || head_dim % 2 || n_pos < 0)
+        return fail(LCMOE_ERR_INVALID_ARG, "head_dim=%d n_pos=%d", head_dim, n_pos);
+    if (n_pos && !out) return fail(LCMOE_ERR_INVALID_ARG, "out is NULL");
+    for (int32_t i = 0; i < head_dim / 2; i++) {
+        const double f = std::pow((double)theta, -2.0 * i / head_dim);
+        for (int32_t p = 0; p < n_pos; p++) {
+            float *o = out + ((int64_t)p * (head_dim / 2) + i) * 2;
+            o[0] = (float)std::cos(p * f);
+            o[1] = (float)std::sin(p * f);
+        }
+    }
+    return LCMOE_OK;
+}
+
 extern "C" void lcmoe_synth_normal(uint64_t seed, uint64_t stream, float stddev, float *out, int64_t n) {
     if (!out || n <= 0) return;
     const uint64_t G = 0x9E3779B97F4A7C15ULL;
