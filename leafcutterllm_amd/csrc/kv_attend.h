@@ -1,0 +1,676 @@
+// The attention kernel over a paged cache, for both kinds of pages; its
+// instances are in kern_kv_attn_i8.hip and kern_kv_attn_f16.hip, its launches
+// in kern_kv_attn.hip.
+//
+// A block takes M = 16 NT query rows of one K/V head -- (token, query head of
+// the group) pairs, so that grouped heads share the keys they read -- and a
+// range of the context.  Its four waves take steps of ST tokens in turn, each
+// with all M rows, and join at the end; blocks that share rows leave partials
+// for k_attend_join.  A step is
+//   S^T = K Q^T   [16 tokens x 16 rows] per unit of 16 tokens,
+//   p = 2^(S - m) with the running maximum m and sum l,
+//   O^T += V^T P^T  [16 dims x 16 rows] per 16 dims,
+// all on 16x16 matrix instructions.  The lane that holds row r and tokens 4 g
+// .. 4 g + 3 of a unit in S^T holds the same ones as an operand of P^T, so
+// probabilities stay in registers; a unit's layout (kv_device.h) makes every
+// operand of K and V a 16-byte load at lane * 16.
+//
+// 8-bit pages: codes go into integer products as they are (16x16x64, twice the
+// f16 rate, no conversion).  Queries and probabilities become NP signed 8-bit
+// pieces of a fixed-point value, x = sum of piece_i 256^i: 15 bits (NP = 2) of
+// the row's largest for f16 and bf16 activations, 23 bits (NP = 3) for f32.
+// Integer sums are exact; the scales are applied in f32, the keys' to the
+// score, the values' to p, relative to the largest of the step.
+// f16 pages: NP f16 pieces, of q scaled by a power of two, and of p 2^10.
+#pragma once
+
+#include "kv_device.h"
+
+namespace lcmoe {
+
+struct AttendArgs {
+    const void *q;
+    int64_t ldq;
+    const float *rope;
+    float scale;
+    void *out;
+    int64_t ldo;
+    bool vec;
+    int splits;   // blocks that may share a row
+    int per_seq;  // tiles per sequence, all alike; 0: as many as its rows fill
+    int lo, hi;   // sequences with lo < rows <= hi only (rows: tokens * group)
+    float *part_o, *part_ml;
+};
+
+// tokens of a step, and the fewest steps that a block is given
+template <bool I8> constexpr int kStep = I8 ? 64 : 32;
+constexpr int kWaves = 4;
+
+typedef int32_t intx4 __attribute__((ext_vector_type(4)));
+
+// A tile of M rows of one sequence and its share of the context.
+struct Tile {
+    Seq s;
+    int b, r0;       // sequence, first (token, head) row of the tile
+    int rows;        // the sequence's rows
+    int n_tok;       // tokens that some row of the tile sees
+    int all_see;     // tokens that every row sees
+    int steps, per, parts;  // steps, steps per block, blocks with any
+};
+template <bool I8, int M>
+__device__ __forceinline__ bool find_rows(const KvArgs &a, const AttendArgs &t, int tile, Tile &x) {
+    const int G = a.H / a.KVH;
+    int j = 0;
+    if (t.per_seq) {
+        x.b = tile / t.per_seq;
+        j = tile % t.per_seq;
+    } else {
+        x.b = find_tile(a, tile, [&](const Seq &s) {
+            const int rows = max(s.cnt, 0) * G;
+            return rows > t.lo && rows <= t.hi ? (rows + M - 1) / M : 0;
+        }, j);
+        if (x.b < 0) return false;
+    }
+    x.s = sequence(a, x.b);
+    x.rows = max(x.s.cnt, 0) * G;
+    x.r0 = j * M;
+    if (x.r0 >= x.rows || x.rows <= t.lo || x.rows > t.hi) return false;
+    x.all_see = x.s.len0 + x.r0 / G + 1;
+    x.n_tok = x.s.len0 + (min(x.r0 + M, x.rows) - 1) / G + 1;
+    x.steps = (x.n_tok + kStep<I8> - 1) / kStep<I8>;
+    const int parts = min(t.splits, (x.steps + kWaves - 1) / kWaves);
+    x.per = (x.steps + parts - 1) / parts;
+    x.parts = (x.steps + x.per - 1) / x.per;
+    return true;
+}
+
+// over the four lanes that hold a row (lane, lane ^ 16, ^ 32, ^ 48)
+__device__ __forceinline__ float row_max(float v) {
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float row_sum(float v) {
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+__device__ __forceinline__ void load8_any(int act, const void *p, int64_t e, bool vec, float (&o)[8]) {
+    if (act == LCMOE_TYPE_F32) load8<LCMOE_TYPE_F32>(p, e, vec, o);
+    else if (act == LCMOE_TYPE_F16) load8<LCMOE_TYPE_F16>(p, e, vec, o);
+    else load8<LCMOE_TYPE_BF16>(p, e, vec, o);
+}
+// 4 consecutive values
+__device__ __forceinline__ void store4_any(int act, void *p, int64_t e, bool vec, floatx4 v) {
+    if (act == LCMOE_TYPE_F32) {
+        float *o = static_cast<float *>(p) + e;
+        if (vec) *reinterpret_cast<floatx4 *>(o) = v;
+        else
+            for (int i = 0; i < 4; i++) o[i] = v[i];
+    } else {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            w[i] = act == LCMOE_TYPE_F16 ? to16<LCMOE_TYPE_F16>(v[i]) : to_bf16(v[i]);
+        uint16_t *o = static_cast<uint16_t *>(p) + e;
+        if (vec) *reinterpret_cast<uintx2 *>(o) = uintx2{w[0] | (w[1] << 16), w[2] | (w[3] << 16)};
+        else
+            for (int i = 0; i < 4; i++) o[i] = (uint16_t)w[i];
+    }
+}
+
+// byte `B` of four words, as one word
+template <int B>
+__device__ __forceinline__ uint32_t bytes4(const uint32_t (&x)[4]) {
+    constexpr uint32_t pair = 0x0c0c0000u | (uint32_t)(B + 4) << 8 | B;
+    const uint32_t a = __builtin_amdgcn_perm(x[1], x[0], pair);
+    const uint32_t b = __builtin_amdgcn_perm(x[3], x[2], pair);
+    return __builtin_amdgcn_perm(b, a, 0x05040100u);
+}
+
+// The operands of one kind of page, for a head of 32 NS dims.  wide: 16-byte
+// operands of 64 (8 bits) or 32 (f16) dims; tail: the last 32 in 8 bits.
+template <bool I8, int NP, int NS>
+struct Ops;
+
+template <int NP, int NS>
+struct Ops<true, NP, NS> {
+    static constexpr int NJ = NS / 2, TAIL = NS & 1, UN = 4;
+    static constexpr float kQ = NP == 2 ? 127.0f * 256 : 127.0f * 65536;  // most of x
+    struct Unit {
+        uintx4 w[NJ ? NJ : 1];
+        uintx2 tail;
+    };
+    struct Row {  // one row's dims of the lane's group
+        intx4 w[NP][NJ ? NJ : 1];
+        int64_t tail[NP];
+    };
+    __device__ __forceinline__ static void load(Unit &u, const uint8_t *pool, int64_t at, int lane) {
+        const uint8_t *p = pool + at;
+#pragma unroll
+        for (int j = 0; j < NJ; j++)
+            u.w[j] = *reinterpret_cast<const uintx4 *>(p + j * 1024 + lane * 16);
+        if constexpr (TAIL != 0)
+            u.tail = *reinterpret_cast<const uintx2 *>(p + NJ * 1024 + lane * 8);
+    }
+    // pieces of y / most, |y| <= most, for 4 values: piece NP - 1 the lowest
+    __device__ __forceinline__ static void pieces(const float *y, float most, uint32_t (&o)[NP]) {
+        uint32_t x[4], c[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            x[i] = (uint32_t)(int32_t)__builtin_rintf(most > 0.0f ? y[i] / most * kQ : 0.0f);
+        o[NP - 1] = bytes4<0>(x);
+#pragma unroll
+        for (int i = 0; i < 4; i++) c[i] = x[i] + 128u;
+        o[NP - 2] = bytes4<1>(c);
+        if constexpr (NP == 3) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) c[i] = x[i] + 128u + 32768u;
+            o[0] = bytes4<2>(c);
+        }
+    }
+};
+
+template <int NP, int NS>
+struct Ops<false, NP, NS> {
+    static constexpr int NJ = NS, TAIL = 0, UN = 2;
+    struct Unit {
+        half8 w[NJ];
+    };
+    struct Row {
+        half8 w[NP][NJ];
+    };
+    __device__ __forceinline__ static void load(Unit &u, const uint8_t *pool, int64_t at, int lane) {
+        const uint8_t *p = pool + 2 * at;
+#pragma unroll
+        for (int j = 0; j < NJ; j++)
+            u.w[j] = *reinterpret_cast<const half8 *>(p + j * 1024 + lane * 16);
+    }
+};
+
+// The tile's rows of q, rotated: the operands of Q^T, and per row what a
+// score is multiplied by (the row's scale, the call's, and log2 e).
+template <bool I8, int NP, int NS, int NT>
+__device__ __forceinline__ void load_q(const KvArgs &a, const AttendArgs &t, const Tile &x, int h,
+                                       int lane, typename Ops<I8, NP, NS>::Row (&qf)[NT],
+                                       float (&mul)[NT], int (&pos)[NT]) {
+    typedef Ops<I8, NP, NS> O;
+    const int G = a.H / a.KVH, half = a.hd / 2, grp = lane >> 4;
+    constexpr float kLog2e = 1.44269504088896340736f;
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+        const int r = x.r0 + 16 * n + (lane & 15), i = r / G;
+        const bool valid = r < x.rows;
+        // rows past the last see every token and are not stored
+        pos[n] = valid ? x.s.len0 + i : 0x7fffffff;
+        const int64_t e = (int64_t)(x.s.row0 + i) * t.ldq + (int64_t)(h * G + r % G) * a.hd;
+        const float *cs = t.rope + (int64_t)(a.rope_abs ? x.s.len0 + i : i) * a.hd;
+        // dims of the lane's group: 8 bits, 16 of each 64 (and 8 of a last
+        // 32); f16, 8 of each 32
+        float y[NS][8];
+        float most = 0.0f, bad = 0.0f;
+#pragma unroll
+        for (int c = 0; c < NS; c++) {
+            const int d = I8 && c < 2 * (NS / 2) ? 64 * (c / 2) + 16 * grp + 8 * (c % 2)
+                                                 : 32 * c + 8 * grp;
+            if (valid && d < a.hd) {
+                load8_any(a.act, t.q, e + d, t.vec, y[c]);
+                if (t.rope) {
+                    float z[8];
+                    const bool up = d >= half;
+                    load8_any(a.act, t.q, e + (up ? d - half : d + half), t.vec, z);
+                    const float *w = cs + 2 * (up ? d - half : d);
+#pragma unroll
+                    for (int k = 0; k < 8; k++)
+                        y[c][k] = up ? z[k] * w[2 * k + 1] + y[c][k] * w[2 * k]
+                                     : y[c][k] * w[2 * k] - z[k] * w[2 * k + 1];
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < 8; k++) y[c][k] = 0.0f;
+            }
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                most = fmaxf(most, fabsf(y[c][k]));
+                bad = __builtin_fmaf(y[c][k], 0.0f, bad);  // NaN where y is not finite
+            }
+        }
+        most = row_max(most);
+        bad = row_sum(bad);
+        if constexpr (I8) {
+            mul[n] = most * t.scale * (kLog2e / O::kQ) + bad;
+#pragma unroll
+            for (int c = 0; c < NS; c++) {
+                uint32_t o0[NP], o1[NP];
+                O::pieces(&y[c][0], most, o0);
+                O::pieces(&y[c][4], most, o1);
+#pragma unroll
+                for (int p = 0; p < NP; p++) {
+                    if (c < 2 * (NS / 2)) {
+                        qf[n].w[p][c / 2][2 * (c % 2)] = (int)o0[p];
+                        qf[n].w[p][c / 2][2 * (c % 2) + 1] = (int)o1[p];
+                    } else {
+                        qf[n].tail[p] = (int64_t)(((uint64_t)o1[p] << 32) | o0[p]);
+                    }
+                }
+            }
+        } else {
+            // the row's largest to [2^14, 2^15): pieces are normal f16 values
+            const int ex = most > 0.0f && most < INFINITY ? __builtin_amdgcn_frexp_expf(most) : 0;
+            mul[n] = __builtin_amdgcn_ldexpf(t.scale, ex - 15) * kLog2e + bad;
+#pragma unroll
+            for (int c = 0; c < NS; c++)
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    const float v = __builtin_amdgcn_ldexpf(y[c][k], 15 - ex);
+                    const _Float16 hi = (_Float16)v;
+                    qf[n].w[0][c][k] = hi;
+                    if constexpr (NP == 2) qf[n].w[1][c][k] = (_Float16)(v - (float)hi);
+                }
+        }
+    }
+}
+
+template <bool I8, int NP, int NS, int NT>
+__global__ __launch_bounds__(256) void k_attend(KvArgs a, AttendArgs t) {
+    typedef Ops<I8, NP, NS> O;
+    constexpr int M = 16 * NT, HDP = 32 * NS, UN = O::UN, ST = kStep<I8>, TD = HDP / 16;
+    const int lane = threadIdx.x & 63, grp = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int h = blockIdx.x % a.KVH, split = blockIdx.y;
+    Tile x;
+    // the last tiles first: a prompt's see the most
+    if (!find_rows<I8, M>(a, t, gridDim.x / a.KVH - 1 - blockIdx.x / a.KVH, x)) return;
+    if (split >= x.parts) return;
+    typename O::Row qf[NT];
+    float mul[NT];
+    int pos[NT];
+    load_q<I8, NP, NS, NT>(a, t, x, h, lane, qf, mul, pos);
+
+    const int step0 = split * x.per + wave, step1 = min(x.steps, (split + 1) * x.per);
+    const int last_unit = (x.n_tok - 1) >> 4, ushift = a.plog - 4;
+    const int32_t *table = a.pages + (int64_t)x.b * a.max_pages;
+    // pages and scales of the next 64 units that this wave meets, one a lane
+    int m_page = -1;
+    float m_ks = 0.0f, m_vs = 0.0f;
+    const auto fetch_meta = [&](int step) {
+        const int unit = min((step + kWaves * (lane / UN)) * UN + lane % UN, last_unit);
+        m_page = table[unit >> ushift];
+        if (m_page < 0 || m_page >= a.n_pages) m_page = -1;
+        if constexpr (I8) {
+            const float *s = a.scale + ((int64_t)max(m_page, 0) * a.KVH + h) * 2;
+            m_ks = m_page < 0 ? 0.0f : s[0];
+            m_vs = m_page < 0 ? 0.0f : s[1];
+        }
+    };
+    // place of unit u of the wave's step `step`, `in` steps after the fetch
+    const auto place = [&](int step, int in, int u) {
+        const int page = max(__builtin_amdgcn_readlane(m_page, in * UN + u), 0);
+        const int unit = min(step * UN + u, last_unit) & ((1 << ushift) - 1);
+        return unit_base(a, page, h, unit);
+    };
+
+    floatx4 acc[NT][TD];
+    float m[NT], l[NT];
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+        m[n] = -INFINITY;
+        l[n] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < TD; d++) acc[n][d] = floatx4{0, 0, 0, 0};
+    }
+    typename O::Unit kf[UN], vf[UN];
+    int in = 0;
+    if (step0 < step1) {
+        fetch_meta(step0);
+#pragma unroll
+        for (int u = 0; u < UN; u++) O::load(kf[u], a.k, place(step0, 0, u), lane);
+    }
+    for (int step = step0; step < step1; step += kWaves) {
+        bool there[UN];
+        float ks[UN], vs[UN];
+#pragma unroll
+        for (int u = 0; u < UN; u++) {
+            there[u] = __builtin_amdgcn_readlane(m_page, in * UN + u) >= 0;
+            if constexpr (I8) {
+                ks[u] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(m_ks), in * UN + u));
+                vs[u] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(m_vs), in * UN + u));
+            }
+            O::load(vf[u], a.v, place(step, in, u), lane);
+        }
+        bool whole = (step + 1) * ST <= x.all_see;
+#pragma unroll
+        for (int u = 0; u < UN; u++) whole = whole && there[u];
+        // scores
+        float s[NT][UN][4];
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int u = 0; u < UN; u++) {
+                if constexpr (I8) {
+                    intx4 c[NP];
+#pragma unroll
+                    for (int p = 0; p < NP; p++) {
+                        c[p] = intx4{0, 0, 0, 0};
+#pragma unroll
+                        for (int j = 0; j < O::NJ; j++)
+                            c[p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(
+                                __builtin_bit_cast(intx4, kf[u].w[j]), qf[n].w[p][j], c[p], 0, 0, 0);
+                        if constexpr (O::TAIL != 0)
+                            c[p] = __builtin_amdgcn_mfma_i32_16x16x32_i8(
+                                __builtin_bit_cast(int64_t, kf[u].tail), qf[n].tail[p], c[p], 0, 0, 0);
+                    }
+                    const float f = mul[n] * ks[u];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        // |low two| < 2^31: 256 dims of 127 * 127 times 257
+                        float v = (float)((c[NP - 2][e] << 8) + c[NP - 1][e]);
+                        if constexpr (NP == 3) v = __builtin_fmaf((float)c[0][e], 65536.0f, v);
+                        s[n][u][e] = v * f;
+                    }
+                } else {
+                    floatx4 c = {0, 0, 0, 0};
+#pragma unroll
+                    for (int p = 0; p < NP; p++)
+#pragma unroll
+                        for (int j = 0; j < O::NJ; j++)
+                            c = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[u].w[j], qf[n].w[p][j], c,
+                                                                       0, 0, 0);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) s[n][u][e] = c[e] * mul[n];
+                }
+            }
+        // the next step's keys go out before this one's softmax
+        if (step + kWaves < step1) {
+            in++;
+            if (in == 64 / UN) {
+                in = 0;
+                fetch_meta(step + kWaves);
+            }
+#pragma unroll
+            for (int u = 0; u < UN; u++)
+                O::load(kf[u], a.k, place(step + kWaves, in, u), lane);
+        }
+        if (!whole) {
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int u = 0; u < UN; u++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const int tok = step * ST + 16 * u + 4 * grp + e;
+                        if (tok > pos[n] || tok >= x.n_tok || !there[u]) s[n][u][e] = -INFINITY;
+                    }
+        }
+        // values that no row may meet, and those that not every row may
+        bool odd = false;
+        if constexpr (!I8) {
+            if (!whole) {
+#pragma unroll
+                for (int u = 0; u < UN; u++)
+#pragma unroll
+                    for (int j = 0; j < O::NJ; j++)
+#pragma unroll
+                        for (int k = 0; k < 8; k++) {
+                            const int tok = step * ST + 16 * u + 4 * grp + k % 4;
+                            if (tok >= x.n_tok || !there[u]) vf[u].w[j][k] = (_Float16)0.0f;
+                            const _Float16 z = vf[u].w[j][k] * (_Float16)0.0f;
+                            odd = odd || z != z;
+                        }
+                odd = __ballot(odd) != 0;
+            }
+        }
+        float vmax = 0.0f, vmul = 0.0f, ratio[UN];
+        if constexpr (I8) {
+#pragma unroll
+            for (int u = 0; u < UN; u++) vmax = fmaxf(vmax, vs[u]);
+            // a reciprocal that neither overflows nor is lost
+            const float big = vmax < 0x1p-100f ? 0x1p100f : 1.0f;
+            const float inv = vmax > 0.0f ? __builtin_amdgcn_rcpf(vmax * big) : 0.0f;
+#pragma unroll
+            for (int u = 0; u < UN; u++) ratio[u] = vs[u] * big * inv * O::kQ;
+            vmul = vmax * (1.0f / O::kQ);
+        }
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            float mx = -INFINITY;
+#pragma unroll
+            for (int u = 0; u < UN; u++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) mx = fmaxf(mx, s[n][u][e]);
+            mx = fmaxf(m[n], row_max(mx));
+            const float base = mx == -INFINITY ? 0.0f : mx;
+            const float keep = __builtin_amdgcn_exp2f(m[n] - base);
+            m[n] = mx;
+            float sum = 0.0f;
+#pragma unroll
+            for (int u = 0; u < UN; u++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    s[n][u][e] = __builtin_amdgcn_exp2f(s[n][u][e] - (I8 ? base : base - 10.0f));
+                    sum += s[n][u][e];
+                }
+            l[n] = __builtin_fmaf(l[n], keep, sum);
+            if (__ballot(keep != 1.0f)) {
+#pragma unroll
+                for (int d = 0; d < TD; d++) acc[n][d] *= keep;
+            }
+            if constexpr (I8) {
+                intx4 pf[NP];
+#pragma unroll
+                for (int u = 0; u < UN; u++) {
+                    uint32_t b[4], c[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++)  // the fraction's bits: p ratio, rounded
+                        b[e] = __float_as_uint(__builtin_fmaf(s[n][u][e], ratio[u], 8388608.0f));
+                    pf[NP - 1][u] = (int)bytes4<0>(b);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) c[e] = b[e] + 128u;
+                    pf[NP - 2][u] = (int)bytes4<1>(c);
+                    if constexpr (NP == 3) {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) c[e] = b[e] + 128u + 32768u;
+                        pf[0][u] = (int)bytes4<2>(c);
+                    }
+                }
+#pragma unroll
+                for (int d = 0; d < TD; d++) {
+                    intx4 va, c[NP];
+#pragma unroll
+                    for (int u = 0; u < UN; u++)
+                        va[u] = d < 4 * O::NJ ? (int)vf[u].w[O::NJ ? d / 4 : 0][d % 4]
+                                              : (int)vf[u].tail[d % 2];
+#pragma unroll
+                    for (int p = 0; p < NP; p++)
+                        c[p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(va, pf[p], intx4{0, 0, 0, 0}, 0,
+                                                                     0, 0);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const float v = (float)((c[NP - 2][e] << 8) + c[NP - 1][e]);
+                        acc[n][d][e] = __builtin_fmaf(v, vmul, acc[n][d][e]);
+                        if constexpr (NP == 3)
+                            acc[n][d][e] = __builtin_fmaf((float)c[0][e], vmul * 65536.0f, acc[n][d][e]);
+                    }
+                }
+            } else {
+                half8 pf[NP];
+#pragma unroll
+                for (int u = 0; u < UN; u++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const _Float16 hi = (_Float16)s[n][u][e];
+                        pf[0][4 * u + e] = hi;
+                        if constexpr (NP == 2) pf[1][4 * u + e] = (_Float16)(s[n][u][e] - (float)hi);
+                    }
+#pragma unroll
+                for (int d = 0; d < TD; d++) {
+                    half8 va;
+#pragma unroll
+                    for (int u = 0; u < UN; u++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) va[4 * u + e] = vf[u].w[d / 2][4 * (d % 2) + e];
+                    if (odd) {
+                        // values that are not finite meet only the rows that
+                        // see them, whose sums they leave NaN
+                        half8 see, is;
+#pragma unroll
+                        for (int k = 0; k < 8; k++) {
+                            const int tok = step * ST + 16 * (k / 4) + 4 * grp + k % 4;
+                            const _Float16 z = va[k] * (_Float16)0.0f;
+                            is[k] = z == z ? (_Float16)0.0f : (_Float16)1.0f;
+                            va[k] = z == z ? va[k] : (_Float16)0.0f;
+                            see[k] = tok <= pos[n] ? (_Float16)1.0f : (_Float16)0.0f;
+                        }
+                        const floatx4 c = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                            is, see, floatx4{0, 0, 0, 0}, 0, 0, 0);
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            if (c[e] > 0.0f) acc[n][d][e] = NAN;
+                    }
+#pragma unroll
+                    for (int p = 0; p < NP; p++)
+                        acc[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pf[p], acc[n][d], 0, 0,
+                                                                           0);
+                }
+            }
+        }
+    }
+
+    // the four waves' sums, in units of 2^(their largest maximum)
+    __shared__ float s_m[kWaves][M], s_l[kWaves][M];
+    __shared__ __attribute__((aligned(16))) float s_o[kWaves / 2][M][HDP + 4];
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+        l[n] = row_sum(l[n]);
+        if (lane < 16) {
+            s_m[wave][16 * n + lane] = m[n];
+            s_l[wave][16 * n + lane] = l[n];
+        }
+    }
+    __syncthreads();
+    float top[NT];
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+        const int r = 16 * n + (lane & 15);
+        top[n] = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWaves; w++) top[n] = fmaxf(top[n], s_m[w][r]);
+        const float base = top[n] == -INFINITY ? 0.0f : top[n];
+        const float f = __builtin_amdgcn_exp2f(m[n] - base);
+        l[n] = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWaves; w++)
+            l[n] = __builtin_fmaf(s_l[w][r], __builtin_amdgcn_exp2f(s_m[w][r] - base), l[n]);
+#pragma unroll
+        for (int d = 0; d < TD; d++) acc[n][d] *= f;
+    }
+#pragma unroll
+    for (int from = kWaves / 2; from >= 1; from /= 2) {
+        if (wave >= from && wave < 2 * from) {
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int d = 0; d < TD; d++)
+                    *reinterpret_cast<floatx4 *>(&s_o[wave - from][16 * n + (lane & 15)][16 * d + 4 * grp]) =
+                        acc[n][d];
+        }
+        __syncthreads();
+        if (wave < from) {
+#pragma unroll
+            for (int n = 0; n < NT; n++)
+#pragma unroll
+                for (int d = 0; d < TD; d++)
+                    acc[n][d] += *reinterpret_cast<const floatx4 *>(
+                        &s_o[wave][16 * n + (lane & 15)][16 * d + 4 * grp]);
+        }
+        __syncthreads();
+    }
+    if (wave) return;
+    const int G = a.H / a.KVH;
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+        const int r = x.r0 + 16 * n + (lane & 15);
+        if (r >= x.rows) continue;
+        const int64_t row = x.s.row0 + r / G;
+        const int head = h * G + r % G;
+        if (x.parts == 1) {
+            const float inv = l[n] == 0.0f ? 0.0f : 1.0f / l[n];
+#pragma unroll
+            for (int d = 0; d < TD; d++)
+                if (16 * d < a.hd)
+                    store4_any(a.act, t.out, row * t.ldo + (int64_t)head * a.hd + 16 * d + 4 * grp,
+                               t.vec, acc[n][d] * inv);
+        } else {
+            const int64_t at = (row * a.H + head) * t.splits + split;
+#pragma unroll
+            for (int d = 0; d < TD; d++)
+                *reinterpret_cast<floatx4 *>(t.part_o + at * HDP + 16 * d + 4 * grp) = acc[n][d];
+            if (lane < 16) {
+                t.part_ml[2 * at] = top[n];
+                t.part_ml[2 * at + 1] = l[n];
+            }
+        }
+    }
+}
+
+// Rows that several blocks shared: their sums in units of 2^(the largest
+// maximum).  A thread takes four dims of a row.
+template <bool I8, int NT>
+__global__ __launch_bounds__(256) void k_attend_join(KvArgs a, AttendArgs t) {
+    constexpr int M = 16 * NT;
+    const int h = blockIdx.x % a.KVH, G = a.H / a.KVH;
+    Tile x;
+    if (!find_rows<I8, M>(a, t, gridDim.x / a.KVH - 1 - blockIdx.x / a.KVH, x)) return;
+    if (x.parts == 1) return;
+    const int C = a.hd / 4;
+    for (int i = blockIdx.y * 256 + threadIdx.x; i < M * C; i += 256 * gridDim.y) {
+        const int r = x.r0 + i / C, d = 4 * (i % C);
+        if (r >= x.rows) break;
+        const int64_t row = x.s.row0 + r / G;
+        const int head = h * G + r % G;
+        const int64_t at = (row * a.H + head) * t.splits;
+        float top = -INFINITY;
+        for (int s = 0; s < x.parts; s++) top = fmaxf(top, t.part_ml[2 * (at + s)]);
+        const float base = top == -INFINITY ? 0.0f : top;
+        floatx4 o = {0, 0, 0, 0};
+        float l = 0.0f;
+        for (int s = 0; s < x.parts; s++) {
+            const float f = __builtin_amdgcn_exp2f(t.part_ml[2 * (at + s)] - base);
+            l = __builtin_fmaf(t.part_ml[2 * (at + s) + 1], f, l);
+            o += *reinterpret_cast<const floatx4 *>(t.part_o + (at + s) * a.hdp + d) * f;
+        }
+        store4_any(a.act, t.out, row * t.ldo + (int64_t)head * a.hd + d, t.vec,
+                   o * (l == 0.0f ? 0.0f : 1.0f / l));
+    }
+}
+
+// One launch over `tiles` tiles of 16 NT rows, NT 1 or kBigTile, and the join
+// where blocks share rows.
+constexpr int kBigTile = 2;
+hipError_t attend_i8(const KvArgs &a, const AttendArgs &t, int tiles, bool big, hipStream_t st);
+hipError_t attend_f16(const KvArgs &a, const AttendArgs &t, int tiles, bool big, hipStream_t st);
+
+template <bool I8, int NP, int NT>
+hipError_t attend_launch(const KvArgs &a, const AttendArgs &t, int tiles, hipStream_t st) {
+    const dim3 grid((unsigned)tiles * a.KVH, t.splits);
+    const auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(256), 0, st, a, t); };
+    switch (a.hdp / 32) {
+    case 1: go(k_attend<I8, NP, 1, NT>); break;
+    case 2: go(k_attend<I8, NP, 2, NT>); break;
+    case 3: go(k_attend<I8, NP, 3, NT>); break;
+    case 4: go(k_attend<I8, NP, 4, NT>); break;
+    case 5: go(k_attend<I8, NP, 5, NT>); break;
+    case 6: go(k_attend<I8, NP, 6, NT>); break;
+    case 7: go(k_attend<I8, NP, 7, NT>); break;
+    default: go(k_attend<I8, NP, 8, NT>); break;
+    }
+    if (t.splits > 1)
+        hipLaunchKernelGGL((k_attend_join<I8, NT>), dim3((unsigned)tiles * a.KVH, NT * 2), dim3(256), 0,
+                           st, a, t);
+    return hipGetLastError();
+}
+
+}  // namespace lcmoe

@@ -87,6 +87,14 @@ lcmoe_status check_batch(const lcmoe_kv_batch *b, bool arrays) {
     return LCMOE_OK;
 }
 
+// the attention counts its rows, a (token, head) each, in 31 bits
+lcmoe_status check_attended(const lcmoe_kv_desc *d, const lcmoe_kv_batch *b) {
+    if (((int64_t)b->n_rows + b->n_seq) * d->n_head > INT32_MAX)
+        return fail(LCMOE_ERR_INVALID_ARG, "n_rows=%d (and n_seq=%d) of n_head=%d: more than 2^31",
+                    b->n_rows, b->n_seq, d->n_head);
+    return LCMOE_OK;
+}
+
 lcmoe_status check_pool(const lcmoe_kv_desc *d, const lcmoe_kv_pool *p) {
     if (!p || !p->k || !p->v) return fail(LCMOE_ERR_INVALID_ARG, "pool, its k or its v is NULL");
     if (((uintptr_t)p->k | (uintptr_t)p->v) & 15)
@@ -212,6 +220,7 @@ extern "C" lcmoe_status lcmoe_kv_attention_workspace(const lcmoe_kv_desc *desc,
     if (!bytes) return fail(LCMOE_ERR_INVALID_ARG, "bytes is NULL");
     if (lcmoe_status s = check_desc(desc)) return s;
     if (lcmoe_status s = check_batch(batch, false)) return s;
+    if (lcmoe_status s = check_attended(desc, batch)) return s;
     *bytes = nothing(batch) ? 0 : 4 * (size_t)kv_attention_floats(args_of(desc, nullptr, batch));
     return LCMOE_OK;
 }
@@ -224,6 +233,7 @@ extern "C" lcmoe_status lcmoe_kv_attention_dev(const lcmoe_kv_desc *desc, const 
     clear_error();
     if (lcmoe_status s = check_desc(desc)) return s;
     if (lcmoe_status s = check_batch(batch, true)) return s;
+    if (lcmoe_status s = check_attended(desc, batch)) return s;
     if (!(scale > 0.0f) || !std::isfinite(scale))
         return fail(LCMOE_ERR_INVALID_ARG, "scale must be finite and > 0");
     if (nothing(batch)) return LCMOE_OK;

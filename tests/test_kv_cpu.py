@@ -1,5 +1,7 @@
 """The paged cache's and the log probabilities' host side: sizes, the rope
 table and every refusal, before any device work."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
@@ -104,6 +106,25 @@ def test_operand_refusals():
     refused(1, attention, q=FAKE + 3)
     for s in (0.0, -1.0, float("inf"), float("nan")):
         refused(1, attention, scale=s)
+
+
+def test_workspace_refusals():
+    # a long document's token: several blocks share a head, so partials go
+    # through the workspace
+    d, b = desc(max_pages=8192, n_pages=8192), batch(n_seq=1, n_rows=1, max_new=1)
+    n = L.kv_attention_workspace(d, b)
+    assert n > 0
+    # it depends on the sizes alone
+    assert n == L.kv_attention_workspace(d, L.KvBatch(n_seq=1, n_rows=1, max_new=1))
+    refused(1, attention, d, b=b, ws=None)
+    refused(1, attention, d, b=b, n=n - 1)
+    refused(1, attention, d, b=b, ws=FAKE + 8, n=n)
+    assert L.lib().lcmoe_kv_attention_workspace(C.byref(d), C.byref(b), None) == 1
+
+
+def test_attention_too_many_rows():
+    refused(1, attention, b=batch(n_rows=(1 << 30) - 1, max_new=3))
+    refused(1, L.kv_attention_workspace, desc(), batch(n_rows=(1 << 30) - 1, max_new=3))
 
 
 @pytest.mark.parametrize("kw", [dict(n_seq=0, n_rows=0, max_new=0), dict(n_rows=0), dict(max_new=0)])
