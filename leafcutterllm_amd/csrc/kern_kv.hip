@@ -172,11 +172,11 @@ __global__ __launch_bounds__(256) void k_kv_append(KvArgs a, const void *__restr
             }
         }
         // the dims that pad the head to hdp meet zeros of the query: zeros too
-        if (hdp > hd)
-            for (int i = tid; i < 16 * n; i += 256) {
-                const int slot = slot0 + i / 16;
+        if (const int pad = hdp - hd)
+            for (int i = tid; i < pad * n; i += 256) {
+                const int slot = slot0 + i / pad;
                 const int64_t at = (int64_t)(slot >> 4) * 16 * hdp +
-                                   k_place<I8>(hdp, slot & 15, hd + i % 16);
+                                   k_place<I8>(hdp, slot & 15, hd + i % pad);
                 if constexpr (I8) p8[at] = 0;
                 else p16[at] = (_Float16)0.0f;
             }

@@ -8,12 +8,13 @@ namespace lcmoe {
 namespace {
 
 struct Plan {
-    int tiles, splits, per_seq, lo, hi;
+    int tiles, splits, per_seq, lo, hi, waves;  // waves 0: tiles of 16 rows
 };
 
-// blocks that share a row's context, so that about `want` blocks run
-int splits_for(const KvArgs &a, int64_t tiles, int want) {
-    const int64_t steps = ((int64_t)a.max_pages << a.plog) / (a.i8 ? 64 : 32) / kWaves;
+// blocks that share a row's context, so that about `want` blocks run and each
+// has `least` steps of `st` tokens
+int splits_for(const KvArgs &a, int64_t tiles, int want, int st, int least) {
+    const int64_t steps = ((int64_t)a.max_pages << a.plog) / ((int64_t)st * least);
     const int64_t most = std::max<int64_t>(1, std::min<int64_t>(128, steps));
     const int64_t base = std::max<int64_t>(1, tiles * a.KVH);
     return (int)std::max<int64_t>(1, std::min<int64_t>(most, (want + base - 1) / base));
@@ -21,23 +22,27 @@ int splits_for(const KvArgs &a, int64_t tiles, int want) {
 
 // One launch (n = 1) or two: sequences of up to 16 rows, and those of more.
 int plans(const KvArgs &a, Plan (&p)[2]) {
-    const int G = a.H / a.KVH, M = 16 * kBigTile;
+    const int G = a.H / a.KVH;
     const int64_t most = (int64_t)a.max_new * G;  // rows of one sequence
     int n = 0;
     if (most <= 16 || (a.starts && a.n_seq > 1)) {
-        p[n] = {a.n_seq, 0, 1, 0, 16};
-        p[n].splits = splits_for(a, a.n_seq, 1024);
+        p[n] = {a.n_seq, 0, 1, 0, 16, 0};
+        p[n].splits = splits_for(a, a.n_seq, 512, a.i8 ? 64 : 32, kWaves);
         n++;
     }
     if (most > 16) {
-        const int per = (int)((most + M - 1) / M);
         const bool alike = !a.starts || a.n_seq == 1;
-        // sequences' rows fill at most this many tiles, one of each in part
-        const int64_t tiles = alike ? (int64_t)per * a.n_seq
-                                    : std::min<int64_t>((int64_t)a.n_rows * G / M + a.n_seq,
-                                                        (int64_t)per * a.n_seq);
-        p[n] = {(int)tiles, 0, alike ? per : 0, n ? 16 : 0, INT32_MAX};
-        p[n].splits = splits_for(a, tiles, 512);
+        const auto tiles = [&](int M) {
+            const int64_t per = (most + M - 1) / M;
+            // sequences' rows fill at most this many tiles, one of each in part
+            return alike ? per * a.n_seq
+                         : std::min<int64_t>((int64_t)a.n_rows * G / M + a.n_seq, per * a.n_seq);
+        };
+        int w = a.hdp <= 128 ? 8 : 4;
+        if (w == 8 && tiles(32 * w) * a.KVH < 256) w = 2;
+        const int M = 32 * w;
+        p[n] = {(int)tiles(M), 0, alike ? (int)((most + M - 1) / M) : 0, n ? 16 : 0, INT32_MAX, w};
+        p[n].splits = splits_for(a, p[n].tiles, 256, 64, 4);
         n++;
     }
     return n;
@@ -61,9 +66,11 @@ hipError_t launch_kv_attention(const KvArgs &a, const void *q, int64_t ldq, cons
     for (int i = 0, n = plans(a, p); i < n; i++) {
         AttendArgs t{q, ldq, rope, scale, out, ldo, vec, p[i].splits, p[i].per_seq, p[i].lo,
                      p[i].hi, ws, ws + (int64_t)a.n_rows * a.H * p[i].splits * a.hdp};
-        const bool big = p[i].hi > 16;
-        const hipError_t e = a.i8 ? attend_i8(a, t, p[i].tiles, big, st)
-                                  : attend_f16(a, t, p[i].tiles, big, st);
+        if ((int64_t)p[i].tiles * a.KVH > INT32_MAX) return hipErrorInvalidConfiguration;
+        const hipError_t e = !p[i].waves ? (a.i8 ? attend_i8 : attend_f16)(a, t, p[i].tiles, st)
+                             : (a.act == LCMOE_TYPE_F32   ? prompt_f32
+                                : a.act == LCMOE_TYPE_F16 ? prompt_f16
+                                                          : prompt_bf16)(a, t, p[i].tiles, p[i].waves, st);
         if (e != hipSuccess) return e;
     }
     return hipSuccess;

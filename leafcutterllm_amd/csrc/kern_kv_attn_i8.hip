@@ -4,12 +4,9 @@
 
 namespace lcmoe {
 
-hipError_t attend_i8(const KvArgs &a, const AttendArgs &t, int tiles, bool big, hipStream_t st) {
-    if (a.act == LCMOE_TYPE_F32)
-        return big ? attend_launch<true, 3, kBigTile>(a, t, tiles, st)
-                   : attend_launch<true, 3, 1>(a, t, tiles, st);
-    return big ? attend_launch<true, 2, kBigTile>(a, t, tiles, st)
-               : attend_launch<true, 2, 1>(a, t, tiles, st);
+hipError_t attend_i8(const KvArgs &a, const AttendArgs &t, int tiles, hipStream_t st) {
+    return a.act == LCMOE_TYPE_F32 ? attend_launch<true, 3>(a, t, tiles, st)
+                                   : attend_launch<true, 2>(a, t, tiles, st);
 }
 
 }  // namespace lcmoe

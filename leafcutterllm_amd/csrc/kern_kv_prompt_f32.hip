@@ -1,0 +1,11 @@
+// Instances of the prompts' attention for f32 activations (kv_prompt.h).
+
+#include "kv_prompt.h"
+
+namespace lcmoe {
+
+hipError_t prompt_f32(const KvArgs &a, const AttendArgs &t, int tiles, int waves, hipStream_t st) {
+    return prompt_launch<LCMOE_TYPE_F32>(a, t, tiles, waves, st);
+}
+
+}  // namespace lcmoe

@@ -253,7 +253,7 @@ struct KvArgs {
     float *scale;  // [n_pages][KVH][2] (keys, values); 8 bits only
     const int32_t *starts, *lens, *pages;
     int n_seq, n_rows, max_new;
-    int H, KVH, hd, hdp;  // hdp: head_dim rounded up to 32
+    int H, KVH, hd, hdp;  // hdp: head_dim rounded up to 32 (64 past 128)
     int plog;             // log2 of the tokens per page
     int n_pages, max_pages, rope_abs, act;
     bool i8;

@@ -57,7 +57,8 @@ struct Tile {
     int all_see;     // tokens that every row sees
     int steps, per, parts;  // steps, steps per block, blocks with any
 };
-template <bool I8, int M>
+// ST: tokens of a step; LEAST: steps that a block is worth
+template <int ST, int M, int LEAST>
 __device__ __forceinline__ bool find_rows(const KvArgs &a, const AttendArgs &t, int tile, Tile &x) {
     const int G = a.H / a.KVH;
     int j = 0;
@@ -77,8 +78,8 @@ __device__ __forceinline__ bool find_rows(const KvArgs &a, const AttendArgs &t, 
     if (x.r0 >= x.rows || x.rows <= t.lo || x.rows > t.hi) return false;
     x.all_see = x.s.len0 + x.r0 / G + 1;
     x.n_tok = x.s.len0 + (min(x.r0 + M, x.rows) - 1) / G + 1;
-    x.steps = (x.n_tok + kStep<I8> - 1) / kStep<I8>;
-    const int parts = min(t.splits, (x.steps + kWaves - 1) / kWaves);
+    x.steps = (x.n_tok + ST - 1) / ST;
+    const int parts = min(t.splits, (x.steps + LEAST - 1) / LEAST);
     x.per = (x.steps + parts - 1) / parts;
     x.parts = (x.steps + x.per - 1) / x.per;
     return true;
@@ -283,7 +284,7 @@ __global__ __launch_bounds__(256) void k_attend(KvArgs a, AttendArgs t) {
     const int h = blockIdx.x % a.KVH, split = blockIdx.y;
     Tile x;
     // the last tiles first: a prompt's see the most
-    if (!find_rows<I8, M>(a, t, gridDim.x / a.KVH - 1 - blockIdx.x / a.KVH, x)) return;
+    if (!find_rows<ST, M, kWaves>(a, t, gridDim.x / a.KVH - 1 - blockIdx.x / a.KVH, x)) return;
     if (split >= x.parts) return;
     typename O::Row qf[NT];
     float mul[NT];
@@ -617,60 +618,88 @@ __global__ __launch_bounds__(256) void k_attend(KvArgs a, AttendArgs t) {
 }
 
 // Rows that several blocks shared: their sums in units of 2^(the largest
-// maximum).  A thread takes four dims of a row.
-template <bool I8, int NT>
+// maximum).  A block takes one row; groups of hdp / 4 threads, four dims each,
+// take the parts in turn and add up in LDS.
+template <int ST, int M, int LEAST>
 __global__ __launch_bounds__(256) void k_attend_join(KvArgs a, AttendArgs t) {
-    constexpr int M = 16 * NT;
-    const int h = blockIdx.x % a.KVH, G = a.H / a.KVH;
+    __shared__ __attribute__((aligned(16))) floatx4 s_o[256];
+    __shared__ float s_f[128], s_l[128];
+    const int h = blockIdx.x % a.KVH, G = a.H / a.KVH, tid = threadIdx.x;
     Tile x;
-    if (!find_rows<I8, M>(a, t, gridDim.x / a.KVH - 1 - blockIdx.x / a.KVH, x)) return;
-    if (x.parts == 1) return;
-    const int C = a.hd / 4;
-    for (int i = blockIdx.y * 256 + threadIdx.x; i < M * C; i += 256 * gridDim.y) {
-        const int r = x.r0 + i / C, d = 4 * (i % C);
-        if (r >= x.rows) break;
-        const int64_t row = x.s.row0 + r / G;
-        const int head = h * G + r % G;
-        const int64_t at = (row * a.H + head) * t.splits;
-        float top = -INFINITY;
-        for (int s = 0; s < x.parts; s++) top = fmaxf(top, t.part_ml[2 * (at + s)]);
-        const float base = top == -INFINITY ? 0.0f : top;
-        floatx4 o = {0, 0, 0, 0};
-        float l = 0.0f;
-        for (int s = 0; s < x.parts; s++) {
-            const float f = __builtin_amdgcn_exp2f(t.part_ml[2 * (at + s)] - base);
-            l = __builtin_fmaf(t.part_ml[2 * (at + s) + 1], f, l);
-            o += *reinterpret_cast<const floatx4 *>(t.part_o + (at + s) * a.hdp + d) * f;
-        }
-        store4_any(a.act, t.out, row * t.ldo + (int64_t)head * a.hd + d, t.vec,
-                   o * (l == 0.0f ? 0.0f : 1.0f / l));
+    if (!find_rows<ST, M, LEAST>(a, t, gridDim.x / a.KVH - 1 - blockIdx.x / a.KVH, x)) return;
+    const int r = x.r0 + blockIdx.y;
+    if (x.parts == 1 || r >= x.rows) return;
+    const int64_t row = x.s.row0 + r / G;
+    const int head = h * G + r % G;
+    const int64_t at = (row * a.H + head) * t.splits;
+    if (tid < x.parts) {
+        s_f[tid] = t.part_ml[2 * (at + tid)];
+        s_l[tid] = t.part_ml[2 * (at + tid) + 1];
+    }
+    __syncthreads();
+    float top = -INFINITY;
+    for (int s = 0; s < x.parts; s++) top = fmaxf(top, s_f[s]);
+    const float base = top == -INFINITY ? 0.0f : top;
+    __syncthreads();
+    if (tid < x.parts) {
+        s_f[tid] = __builtin_amdgcn_exp2f(s_f[tid] - base);
+        s_l[tid] *= s_f[tid];
+    }
+    __syncthreads();
+    const int C = a.hdp / 4, groups = 256 / C, grp = tid / C, d = 4 * (tid % C);
+    floatx4 o = {0, 0, 0, 0};
+    if (grp < groups) {
+        const float *p = t.part_o + at * a.hdp + d;
+#pragma unroll 4
+        for (int s = grp; s < x.parts; s += groups)
+            o += *reinterpret_cast<const floatx4 *>(p + (int64_t)s * a.hdp) * s_f[s];
+    }
+    s_o[tid] = o;
+    __syncthreads();
+    if (grp || d >= a.hd) return;
+    for (int k = 1; k < groups; k++) o += s_o[k * C + tid];
+    float l = 0.0f;
+    for (int s = 0; s < x.parts; s++) l += s_l[s];
+    store4_any(a.act, t.out, row * t.ldo + (int64_t)head * a.hd + d, t.vec,
+               o * (l == 0.0f ? 0.0f : 1.0f / l));
+}
+
+// Launches over `tiles` tiles: of 16 rows (attend_*), or of 32 W rows, W waves
+// (prompt_*), with the join where blocks share rows.
+hipError_t attend_i8(const KvArgs &a, const AttendArgs &t, int tiles, hipStream_t st);
+hipError_t attend_f16(const KvArgs &a, const AttendArgs &t, int tiles, hipStream_t st);
+hipError_t prompt_f32(const KvArgs &a, const AttendArgs &t, int tiles, int waves, hipStream_t st);
+hipError_t prompt_f16(const KvArgs &a, const AttendArgs &t, int tiles, int waves, hipStream_t st);
+hipError_t prompt_bf16(const KvArgs &a, const AttendArgs &t, int tiles, int waves, hipStream_t st);
+
+template <int ST, int M, int LEAST>
+hipError_t attend_join(const KvArgs &a, const AttendArgs &t, int tiles, hipStream_t st) {
+    if (t.splits > 1)
+        hipLaunchKernelGGL((k_attend_join<ST, M, LEAST>), dim3((unsigned)tiles * a.KVH, M), dim3(256),
+                           0, st, a, t);
+    return hipGetLastError();
+}
+
+// f(the head's 32 dims, as a constant)
+template <class F>
+void by_dims(const KvArgs &a, F f) {
+    switch (a.hdp / 32) {
+    case 1: f(std::integral_constant<int, 1>()); break;
+    case 2: f(std::integral_constant<int, 2>()); break;
+    case 3: f(std::integral_constant<int, 3>()); break;
+    case 4: f(std::integral_constant<int, 4>()); break;
+    case 6: f(std::integral_constant<int, 6>()); break;
+    default: f(std::integral_constant<int, 8>()); break;
     }
 }
 
-// One launch over `tiles` tiles of 16 NT rows, NT 1 or kBigTile, and the join
-// where blocks share rows.
-constexpr int kBigTile = 2;
-hipError_t attend_i8(const KvArgs &a, const AttendArgs &t, int tiles, bool big, hipStream_t st);
-hipError_t attend_f16(const KvArgs &a, const AttendArgs &t, int tiles, bool big, hipStream_t st);
-
-template <bool I8, int NP, int NT>
+template <bool I8, int NP>
 hipError_t attend_launch(const KvArgs &a, const AttendArgs &t, int tiles, hipStream_t st) {
-    const dim3 grid((unsigned)tiles * a.KVH, t.splits);
-    const auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(256), 0, st, a, t); };
-    switch (a.hdp / 32) {
-    case 1: go(k_attend<I8, NP, 1, NT>); break;
-    case 2: go(k_attend<I8, NP, 2, NT>); break;
-    case 3: go(k_attend<I8, NP, 3, NT>); break;
-    case 4: go(k_attend<I8, NP, 4, NT>); break;
-    case 5: go(k_attend<I8, NP, 5, NT>); break;
-    case 6: go(k_attend<I8, NP, 6, NT>); break;
-    case 7: go(k_attend<I8, NP, 7, NT>); break;
-    default: go(k_attend<I8, NP, 8, NT>); break;
-    }
-    if (t.splits > 1)
-        hipLaunchKernelGGL((k_attend_join<I8, NT>), dim3((unsigned)tiles * a.KVH, NT * 2), dim3(256), 0,
-                           st, a, t);
-    return hipGetLastError();
+    by_dims(a, [&](auto ns) {
+        hipLaunchKernelGGL((k_attend<I8, NP, decltype(ns)::value, 1>),
+                           dim3((unsigned)tiles * a.KVH, t.splits), dim3(256), 0, st, a, t);
+    });
+    return attend_join<kStep<I8>, 16, kWaves>(a, t, tiles, st);
 }
 
 }  // namespace lcmoe

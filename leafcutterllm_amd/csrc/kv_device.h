@@ -1,7 +1,8 @@
 // The paged K/V cache's layout and batch, shared by its kernels.
 //
 // A page holds, per K/V head, page_tokens / 16 units of 16 tokens, each 16 *
-// hdp values (hdp: head_dim rounded up to 32) in the order in which a wave of
+// hdp values (hdp: head_dim rounded up to 32, past 128 to
+// 64) in the order in which a wave of
 // the attention feeds its matrix instructions, so that a unit is read with
 // 16-byte loads, 1 KiB in a row:
 //   K, "narrow" (f16, and the last 32 dims in 8 bits when hdp % 64 == 32):

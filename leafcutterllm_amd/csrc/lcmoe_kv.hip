@@ -39,6 +39,9 @@ struct OnDeviceOf {
     }
 };
 
+// the dims a head is held as: a multiple of 32, past 128 one of 64
+int padded_dim(int hd) { return hd <= 128 ? (hd + 31) & ~31 : (hd + 63) & ~63; }
+
 bool act_ok(int t) {
     return t == LCMOE_TYPE_F32 || t == LCMOE_TYPE_F16 || t == LCMOE_TYPE_BF16;
 }
@@ -135,7 +138,7 @@ KvArgs args_of(const lcmoe_kv_desc *d, const lcmoe_kv_pool *p, const lcmoe_kv_ba
     a.H = d->n_head;
     a.KVH = d->n_kv_head;
     a.hd = d->head_dim;
-    a.hdp = (d->head_dim + 31) & ~31;
+    a.hdp = padded_dim(d->head_dim);
     a.plog = __builtin_ctz((unsigned)d->page_tokens);
     a.n_pages = d->n_pages;
     a.max_pages = d->max_pages;
@@ -169,7 +172,7 @@ extern "C" lcmoe_status lcmoe_kv_sizes(const lcmoe_kv_desc *desc, size_t *pool_b
     clear_error();
     if (lcmoe_status s = check_desc(desc)) return s;
     const size_t per_page = (size_t)desc->n_kv_head * desc->page_tokens *
-                            (size_t)((desc->head_dim + 31) & ~31);
+                            (size_t)padded_dim(desc->head_dim);
     const bool i8 = desc->kv_type == LCMOE_TYPE_I8;
     if (pool_bytes) *pool_bytes = per_page * (size_t)desc->n_pages * (i8 ? 1 : 2);
     if (scale_bytes) *scale_bytes = i8 ? 8 * (size_t)desc->n_pages * desc->n_kv_head : 0;
