@@ -8,7 +8,7 @@ namespace lcmoe {
 namespace {
 
 struct Plan {
-    int tiles, splits, per_seq, lo, hi, waves;  // waves 0: tiles of 16 rows
+    int tiles, splits, per_seq, lo, hi, rows;  // rows of a tile
 };
 
 // blocks that share a row's context, so that about `want` blocks run and each
@@ -26,7 +26,7 @@ int plans(const KvArgs &a, Plan (&p)[2]) {
     const int64_t most = (int64_t)a.max_new * G;  // rows of one sequence
     int n = 0;
     if (most <= 16 || (a.starts && a.n_seq > 1)) {
-        p[n] = {a.n_seq, 0, 1, 0, 16, 0};
+        p[n] = {a.n_seq, 0, 1, 0, 16, 16};
         p[n].splits = splits_for(a, a.n_seq, 512, a.i8 ? 64 : 32, kWaves);
         n++;
     }
@@ -38,11 +38,10 @@ int plans(const KvArgs &a, Plan (&p)[2]) {
             return alike ? per * a.n_seq
                          : std::min<int64_t>((int64_t)a.n_rows * G / M + a.n_seq, per * a.n_seq);
         };
-        int w = a.hdp <= 128 ? 8 : 4;
-        if (w == 8 && tiles(32 * w) * a.KVH < 256) w = 2;
-        const int M = 32 * w;
-        p[n] = {(int)tiles(M), 0, alike ? (int)((most + M - 1) / M) : 0, n ? 16 : 0, INT32_MAX, w};
-        p[n].splits = splits_for(a, p[n].tiles, 256, 64, 4);
+        int M = a.hdp <= 128 ? 256 : 128;
+        if (tiles(M) * a.KVH < 96) M = 64;
+        p[n] = {(int)tiles(M), 0, alike ? (int)((most + M - 1) / M) : 0, n ? 16 : 0, INT32_MAX, M};
+        p[n].splits = p[n].tiles * a.KVH > 128 ? 1 : splits_for(a, p[n].tiles, 256, 64, M == 64 ? 16 : 4);
         n++;
     }
     return n;
@@ -67,10 +66,11 @@ hipError_t launch_kv_attention(const KvArgs &a, const void *q, int64_t ldq, cons
         AttendArgs t{q, ldq, rope, scale, out, ldo, vec, p[i].splits, p[i].per_seq, p[i].lo,
                      p[i].hi, ws, ws + (int64_t)a.n_rows * a.H * p[i].splits * a.hdp};
         if ((int64_t)p[i].tiles * a.KVH > INT32_MAX) return hipErrorInvalidConfiguration;
-        const hipError_t e = !p[i].waves ? (a.i8 ? attend_i8 : attend_f16)(a, t, p[i].tiles, st)
-                             : (a.act == LCMOE_TYPE_F32   ? prompt_f32
-                                : a.act == LCMOE_TYPE_F16 ? prompt_f16
-                                                          : prompt_bf16)(a, t, p[i].tiles, p[i].waves, st);
+        const bool many = p[i].rows > 64;
+        const hipError_t e = p[i].rows == 16           ? (a.i8 ? attend_i8 : attend_f16)(a, t, p[i].tiles, st)
+                             : a.act == LCMOE_TYPE_F32 ? prompt_f32(a, t, p[i].tiles, many, st)
+                             : a.act == LCMOE_TYPE_F16 ? prompt_f16(a, t, p[i].tiles, many, st)
+                                                       : prompt_bf16(a, t, p[i].tiles, many, st);
         if (e != hipSuccess) return e;
     }
     return hipSuccess;

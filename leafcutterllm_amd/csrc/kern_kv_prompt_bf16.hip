@@ -4,8 +4,8 @@
 
 namespace lcmoe {
 
-hipError_t prompt_bf16(const KvArgs &a, const AttendArgs &t, int tiles, int waves, hipStream_t st) {
-    return prompt_launch<LCMOE_TYPE_BF16>(a, t, tiles, waves, st);
+hipError_t prompt_bf16(const KvArgs &a, const AttendArgs &t, int tiles, bool many, hipStream_t st) {
+    return prompt_launch<LCMOE_TYPE_BF16>(a, t, tiles, many, st);
 }
 
 }  // namespace lcmoe

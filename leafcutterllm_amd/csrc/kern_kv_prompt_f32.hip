@@ -4,8 +4,8 @@
 
 namespace lcmoe {
 
-hipError_t prompt_f32(const KvArgs &a, const AttendArgs &t, int tiles, int waves, hipStream_t st) {
-    return prompt_launch<LCMOE_TYPE_F32>(a, t, tiles, waves, st);
+hipError_t prompt_f32(const KvArgs &a, const AttendArgs &t, int tiles, bool many, hipStream_t st) {
+    return prompt_launch<LCMOE_TYPE_F32>(a, t, tiles, many, st);
 }
 
 }  // namespace lcmoe

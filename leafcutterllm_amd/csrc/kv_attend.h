@@ -2,7 +2,7 @@
 // instances are in kern_kv_attn_i8.hip and kern_kv_attn_f16.hip, its launches
 // in kern_kv_attn.hip.
 //
-// A block takes M = 16 NT query rows of one K/V head -- (token, query head of
+// A block takes 16 query rows of one K/V head -- (token, query head of
 // the group) pairs, so that grouped heads share the keys they read -- and a
 // range of the context.  Its four waves take steps of ST tokens in turn, each
 // with all M rows, and join at the end; blocks that share rows leave partials
@@ -132,6 +132,23 @@ __device__ __forceinline__ uint32_t bytes4(const uint32_t (&x)[4]) {
     return __builtin_amdgcn_perm(b, a, 0x05040100u);
 }
 
+constexpr float kLog2e = 1.44269504088896340736f;
+
+// f16 pieces of 8 values of a row whose largest is `most`, which comes to
+// [2^14, 2^15), so that the pieces are normal f16 values
+__device__ __forceinline__ int exponent_of(float most) {
+    return most > 0.0f && most < INFINITY ? __builtin_amdgcn_frexp_expf(most) : 0;
+}
+template <int NP>
+__device__ __forceinline__ void half_pieces(const float (&y)[8], int ex, half8 (&o)[NP]) {
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+        const float v = __builtin_amdgcn_ldexpf(y[k], 15 - ex);
+        o[0][k] = (_Float16)v;
+        if constexpr (NP == 2) o[1][k] = (_Float16)(v - (float)o[0][k]);
+    }
+}
+
 // The operands of one kind of page, for a head of 32 NS dims.  wide: 16-byte
 // operands of 64 (8 bits) or 32 (f16) dims; tail: the last 32 in 8 bits.
 template <bool I8, int NP, int NS>
@@ -149,8 +166,33 @@ struct Ops<true, NP, NS> {
         intx4 w[NP][NJ ? NJ : 1];
         int64_t tail[NP];
     };
-    __device__ __forceinline__ static void load(Unit &u, const uint8_t *pool, int64_t at, int lane) {
-        const uint8_t *p = pool + at;
+    // a tile of 16 rows in LDS: [piece][64 dims][lane] of 16 bytes, then [piece][lane] of 8
+    static constexpr int kTile = NP * (NJ * 1024 + TAIL * 512);
+    __device__ __forceinline__ static void put(uint8_t *q, int row, int c, const float (&y)[8], float most) {
+        uint32_t o0[NP], o1[NP];
+        pieces(&y[0], most, o0);
+        pieces(&y[4], most, o1);
+        const bool wide = c < 8 * NJ;
+        const int lane = (wide ? (c & 7) >> 1 : c & 3) * 16 + row;
+        const int at = wide ? (c >> 3) * 1024 + lane * 16 + (c & 1) * 8 : NP * NJ * 1024 + lane * 8;
+#pragma unroll
+        for (int p = 0; p < NP; p++)
+            *reinterpret_cast<uintx2 *>(q + at + p * (wide ? NJ * 1024 : 512)) = uintx2{o0[p], o1[p]};
+    }
+    __device__ __forceinline__ static float factor(float most, float scale) {
+        return most * scale * (kLog2e / kQ);
+    }
+    __device__ __forceinline__ static void take(Row &r, const uint8_t *q, int lane) {
+#pragma unroll
+        for (int p = 0; p < NP; p++) {
+#pragma unroll
+            for (int j = 0; j < NJ; j++)
+                r.w[p][j] = *reinterpret_cast<const intx4 *>(q + (p * NJ + j) * 1024 + lane * 16);
+            if constexpr (TAIL != 0)
+                r.tail[p] = *reinterpret_cast<const int64_t *>(q + NP * NJ * 1024 + p * 512 + lane * 8);
+        }
+    }
+    __device__ __forceinline__ static void load(Unit &u, const uint8_t *p, int lane) {
 #pragma unroll
         for (int j = 0; j < NJ; j++)
             u.w[j] = *reinterpret_cast<const uintx4 *>(p + j * 1024 + lane * 16);
@@ -184,206 +226,194 @@ struct Ops<false, NP, NS> {
     struct Row {
         half8 w[NP][NJ];
     };
-    __device__ __forceinline__ static void load(Unit &u, const uint8_t *pool, int64_t at, int lane) {
-        const uint8_t *p = pool + 2 * at;
+    // a tile of 16 rows in LDS: [piece][32 dims][lane] of 16 bytes
+    static constexpr int kTile = NP * NJ * 1024;
+    __device__ __forceinline__ static void put(uint8_t *q, int row, int c, const float (&y)[8], float most) {
+        half8 o[NP];
+        half_pieces<NP>(y, exponent_of(most), o);
+#pragma unroll
+        for (int p = 0; p < NP; p++)
+            *reinterpret_cast<half8 *>(q + (p * NJ + (c >> 2)) * 1024 + ((c & 3) * 16 + row) * 16) = o[p];
+    }
+    __device__ __forceinline__ static float factor(float most, float scale) {
+        return __builtin_amdgcn_ldexpf(scale, exponent_of(most) - 15) * kLog2e;
+    }
+    __device__ __forceinline__ static void take(Row &r, const uint8_t *q, int lane) {
+#pragma unroll
+        for (int p = 0; p < NP; p++)
+#pragma unroll
+            for (int j = 0; j < NJ; j++)
+                r.w[p][j] = *reinterpret_cast<const half8 *>(q + (p * NJ + j) * 1024 + lane * 16);
+    }
+    __device__ __forceinline__ static void load(Unit &u, const uint8_t *p, int lane) {
 #pragma unroll
         for (int j = 0; j < NJ; j++)
             u.w[j] = *reinterpret_cast<const half8 *>(p + j * 1024 + lane * 16);
     }
 };
 
-// The tile's rows of q, rotated: the operands of Q^T, and per row what a
-// score is multiplied by (the row's scale, the call's, and log2 e).
-template <bool I8, int NP, int NS, int NT>
-__device__ __forceinline__ void load_q(const KvArgs &a, const AttendArgs &t, const Tile &x, int h,
-                                       int lane, typename Ops<I8, NP, NS>::Row (&qf)[NT],
-                                       float (&mul)[NT], int (&pos)[NT]) {
-    typedef Ops<I8, NP, NS> O;
-    const int G = a.H / a.KVH, half = a.hd / 2, grp = lane >> 4;
-    constexpr float kLog2e = 1.44269504088896340736f;
+// A tile's rows of q, rotated, once for a block of T threads: every thread
+// takes 8 dims of a row at a time, as many neighbours as a row has (rounded up
+// to a power of two) find its largest magnitude, and put(row, d / 8, y, most)
+// keeps the 8 values; per row keep(row, most, bad), bad NaN where a value is not
+// finite.  Rows past the sequence's last are zeros.  One loop, for its code is
+// run once and fetched for it.
+template <int NS, int M, int T, class Load, class Put, class Keep>
+__device__ __forceinline__ void stage_q(const KvArgs &a, const AttendArgs &t, const Tile &x, int h,
+                                        Load load, Put put, Keep keep) {
+    constexpr int C = 4 * NS, L = C <= 4 ? 4 : C <= 8 ? 8 : C <= 16 ? 16 : 32;  // lanes of a row
+    const int G = a.H / a.KVH, half = a.hd / 2, d = 8 * (threadIdx.x & (L - 1));
+#pragma unroll 1
+    for (int r = threadIdx.x / L; r < M; r += T / L) {
+        const int rr = x.r0 + r, i = rr / G;
+        float y[8], z[8], most = 0.0f, bad = 0.0f;
 #pragma unroll
-    for (int n = 0; n < NT; n++) {
-        const int r = x.r0 + 16 * n + (lane & 15), i = r / G;
-        const bool valid = r < x.rows;
-        // rows past the last see every token and are not stored
-        pos[n] = valid ? x.s.len0 + i : 0x7fffffff;
-        const int64_t e = (int64_t)(x.s.row0 + i) * t.ldq + (int64_t)(h * G + r % G) * a.hd;
-        const float *cs = t.rope + (int64_t)(a.rope_abs ? x.s.len0 + i : i) * a.hd;
-        // dims of the lane's group: 8 bits, 16 of each 64 (and 8 of a last
-        // 32); f16, 8 of each 32
-        float y[NS][8];
-        float most = 0.0f, bad = 0.0f;
-#pragma unroll
-        for (int c = 0; c < NS; c++) {
-            const int d = I8 && c < 2 * (NS / 2) ? 64 * (c / 2) + 16 * grp + 8 * (c % 2)
-                                                 : 32 * c + 8 * grp;
-            if (valid && d < a.hd) {
-                load8_any(a.act, t.q, e + d, t.vec, y[c]);
-                if (t.rope) {
-                    float z[8];
-                    const bool up = d >= half;
-                    load8_any(a.act, t.q, e + (up ? d - half : d + half), t.vec, z);
-                    const float *w = cs + 2 * (up ? d - half : d);
-#pragma unroll
-                    for (int k = 0; k < 8; k++)
-                        y[c][k] = up ? z[k] * w[2 * k + 1] + y[c][k] * w[2 * k]
-                                     : y[c][k] * w[2 * k] - z[k] * w[2 * k + 1];
-                }
-            } else {
-#pragma unroll
-                for (int k = 0; k < 8; k++) y[c][k] = 0.0f;
-            }
-#pragma unroll
-            for (int k = 0; k < 8; k++) {
-                most = fmaxf(most, fabsf(y[c][k]));
-                bad = __builtin_fmaf(y[c][k], 0.0f, bad);  // NaN where y is not finite
-            }
-        }
-        most = row_max(most);
-        bad = row_sum(bad);
-        if constexpr (I8) {
-            mul[n] = most * t.scale * (kLog2e / O::kQ) + bad;
-#pragma unroll
-            for (int c = 0; c < NS; c++) {
-                uint32_t o0[NP], o1[NP];
-                O::pieces(&y[c][0], most, o0);
-                O::pieces(&y[c][4], most, o1);
-#pragma unroll
-                for (int p = 0; p < NP; p++) {
-                    if (c < 2 * (NS / 2)) {
-                        qf[n].w[p][c / 2][2 * (c % 2)] = (int)o0[p];
-                        qf[n].w[p][c / 2][2 * (c % 2) + 1] = (int)o1[p];
-                    } else {
-                        qf[n].tail[p] = (int64_t)(((uint64_t)o1[p] << 32) | o0[p]);
-                    }
-                }
-            }
-        } else {
-            // the row's largest to [2^14, 2^15): pieces are normal f16 values
-            const int ex = most > 0.0f && most < INFINITY ? __builtin_amdgcn_frexp_expf(most) : 0;
-            mul[n] = __builtin_amdgcn_ldexpf(t.scale, ex - 15) * kLog2e + bad;
-#pragma unroll
-            for (int c = 0; c < NS; c++)
+        for (int k = 0; k < 8; k++) y[k] = 0.0f;
+        if (rr < x.rows && d < a.hd) {
+            const int64_t e = (int64_t)(x.s.row0 + i) * t.ldq + (int64_t)(h * G + rr - i * G) * a.hd;
+            load(e + d, y);
+            if (t.rope) {
+                const bool up = d >= half;
+                const int o = up ? d - half : d;
+                load(e + (up ? o : d + half), z);
+                const float *w = t.rope + (int64_t)(a.rope_abs ? x.s.len0 + i : i) * a.hd + 2 * o;
 #pragma unroll
                 for (int k = 0; k < 8; k++) {
-                    const float v = __builtin_amdgcn_ldexpf(y[c][k], 15 - ex);
-                    const _Float16 hi = (_Float16)v;
-                    qf[n].w[0][c][k] = hi;
-                    if constexpr (NP == 2) qf[n].w[1][c][k] = (_Float16)(v - (float)hi);
+                    const float c = w[2 * k], s = up ? -w[2 * k + 1] : w[2 * k + 1];
+                    y[k] = y[k] * c - z[k] * s;
                 }
+            }
         }
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            most = fmaxf(most, fabsf(y[k]));
+            bad = __builtin_fmaf(y[k], 0.0f, bad);
+        }
+#pragma unroll
+        for (int o = 1; o < L; o <<= 1) {
+            most = fmaxf(most, __shfl_xor(most, o, 64));
+            bad += __shfl_xor(bad, o, 64);
+        }
+        if (d < 8 * C) put(r, d >> 3, y, most);
+        if (d == 0) keep(r, most, bad);
     }
 }
 
-template <bool I8, int NP, int NS, int NT>
+template <bool I8, int NP, int NS>
 __global__ __launch_bounds__(256) void k_attend(KvArgs a, AttendArgs t) {
     typedef Ops<I8, NP, NS> O;
-    constexpr int M = 16 * NT, HDP = 32 * NS, UN = O::UN, ST = kStep<I8>, TD = HDP / 16;
+    constexpr int M = 16, HDP = 32 * NS, UN = O::UN, ST = kStep<I8>, TD = HDP / 16;
+    constexpr int LD = HDP + 4, kSums = kWaves * M * LD * 4;
+    // the rows of q, then the four waves' sums
+    __shared__ __attribute__((aligned(16))) uint8_t s_mem[kSums > O::kTile ? kSums : O::kTile];
+    __shared__ float s_mul[M], s_m[kWaves][M], s_l[kWaves][M];
     const int lane = threadIdx.x & 63, grp = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int h = blockIdx.x % a.KVH, split = blockIdx.y;
+    const int h = blockIdx.x % a.KVH, split = blockIdx.y, G = a.H / a.KVH;
     Tile x;
     // the last tiles first: a prompt's see the most
     if (!find_rows<ST, M, kWaves>(a, t, gridDim.x / a.KVH - 1 - blockIdx.x / a.KVH, x)) return;
     if (split >= x.parts) return;
-    typename O::Row qf[NT];
-    float mul[NT];
-    int pos[NT];
-    load_q<I8, NP, NS, NT>(a, t, x, h, lane, qf, mul, pos);
-
     const int step0 = split * x.per + wave, step1 = min(x.steps, (split + 1) * x.per);
     const int last_unit = (x.n_tok - 1) >> 4, ushift = a.plog - 4;
     const int32_t *table = a.pages + (int64_t)x.b * a.max_pages;
-    // pages and scales of the next 64 units that this wave meets, one a lane
-    int m_page = -1;
+    // of the next 64 units that this wave meets, one a lane: whether their page
+    // is there, its scales, and the unit's place in the pools
+    int m_there = 0;
     float m_ks = 0.0f, m_vs = 0.0f;
+    uint32_t m_lo = 0, m_hi = 0;
     const auto fetch_meta = [&](int step) {
         const int unit = min((step + kWaves * (lane / UN)) * UN + lane % UN, last_unit);
-        m_page = table[unit >> ushift];
-        if (m_page < 0 || m_page >= a.n_pages) m_page = -1;
+        int page = table[unit >> ushift];
+        m_there = page >= 0 && page < a.n_pages;
+        page = m_there ? page : 0;
+        const int64_t at = unit_base(a, page, h, unit & ((1 << ushift) - 1)) * (I8 ? 1 : 2);
+        m_lo = (uint32_t)at;
+        m_hi = (uint32_t)(at >> 32);
         if constexpr (I8) {
-            const float *s = a.scale + ((int64_t)max(m_page, 0) * a.KVH + h) * 2;
-            m_ks = m_page < 0 ? 0.0f : s[0];
-            m_vs = m_page < 0 ? 0.0f : s[1];
+            const float *s = a.scale + ((int64_t)page * a.KVH + h) * 2;
+            m_ks = m_there ? s[0] : 0.0f;
+            m_vs = m_there ? s[1] : 0.0f;
         }
     };
-    // place of unit u of the wave's step `step`, `in` steps after the fetch
-    const auto place = [&](int step, int in, int u) {
-        const int page = max(__builtin_amdgcn_readlane(m_page, in * UN + u), 0);
-        const int unit = min(step * UN + u, last_unit) & ((1 << ushift) - 1);
-        return unit_base(a, page, h, unit);
+    // unit u of the step `in` steps after the fetch
+    const auto load = [&](typename O::Unit &w, const uint8_t *pool, int in, int u) {
+        const uint64_t at = (uint32_t)__builtin_amdgcn_readlane(m_lo, in * UN + u) |
+                            (uint64_t)(uint32_t)__builtin_amdgcn_readlane(m_hi, in * UN + u) << 32;
+        O::load(w, pool + at, lane);
     };
-
-    floatx4 acc[NT][TD];
-    float m[NT], l[NT];
-#pragma unroll
-    for (int n = 0; n < NT; n++) {
-        m[n] = -INFINITY;
-        l[n] = 0.0f;
-#pragma unroll
-        for (int d = 0; d < TD; d++) acc[n][d] = floatx4{0, 0, 0, 0};
-    }
     typename O::Unit kf[UN], vf[UN];
     int in = 0;
-    if (step0 < step1) {
-        fetch_meta(step0);
+    fetch_meta(step0);
 #pragma unroll
-        for (int u = 0; u < UN; u++) O::load(kf[u], a.k, place(step0, 0, u), lane);
-    }
+    for (int u = 0; u < UN; u++) load(kf[u], a.k, 0, u);
+
+    stage_q<NS, M, 256>(a, t, x, h,
+        [&](int64_t e, float (&y)[8]) { load8_any(a.act, t.q, e, t.vec, y); },
+        [&](int row, int c, const float (&y)[8], float most) { O::put(s_mem, row, c, y, most); },
+        [&](int row, float most, float bad) { s_mul[row] = O::factor(most, t.scale) + bad; });
+    __syncthreads();
+    typename O::Row qf;
+    O::take(qf, s_mem, lane);
+    const float mul = s_mul[lane & 15];
+    // rows past the last see every token and are not stored
+    const int r_own = x.r0 + (lane & 15), pos = r_own < x.rows ? x.s.len0 + r_own / G : 0x7fffffff;
+    __syncthreads();  // s_mem is the sums' from here on
+
+    floatx4 acc[TD];
+    float m = -INFINITY, l = 0.0f;
+#pragma unroll
+    for (int d = 0; d < TD; d++) acc[d] = floatx4{0, 0, 0, 0};
     for (int step = step0; step < step1; step += kWaves) {
         bool there[UN];
         float ks[UN], vs[UN];
+        bool whole = (step + 1) * ST <= x.all_see;
 #pragma unroll
         for (int u = 0; u < UN; u++) {
-            there[u] = __builtin_amdgcn_readlane(m_page, in * UN + u) >= 0;
+            there[u] = __builtin_amdgcn_readlane(m_there, in * UN + u) != 0;
+            whole = whole && there[u];
             if constexpr (I8) {
                 ks[u] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(m_ks), in * UN + u));
                 vs[u] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(m_vs), in * UN + u));
             }
-            O::load(vf[u], a.v, place(step, in, u), lane);
+            load(vf[u], a.v, in, u);
         }
-        bool whole = (step + 1) * ST <= x.all_see;
-#pragma unroll
-        for (int u = 0; u < UN; u++) whole = whole && there[u];
         // scores
-        float s[NT][UN][4];
+        float s[UN][4];
 #pragma unroll
-        for (int n = 0; n < NT; n++)
+        for (int u = 0; u < UN; u++) {
+            if constexpr (I8) {
+                intx4 c[NP];
 #pragma unroll
-            for (int u = 0; u < UN; u++) {
-                if constexpr (I8) {
-                    intx4 c[NP];
+                for (int p = 0; p < NP; p++) {
+                    c[p] = intx4{0, 0, 0, 0};
 #pragma unroll
-                    for (int p = 0; p < NP; p++) {
-                        c[p] = intx4{0, 0, 0, 0};
-#pragma unroll
-                        for (int j = 0; j < O::NJ; j++)
-                            c[p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(
-                                __builtin_bit_cast(intx4, kf[u].w[j]), qf[n].w[p][j], c[p], 0, 0, 0);
-                        if constexpr (O::TAIL != 0)
-                            c[p] = __builtin_amdgcn_mfma_i32_16x16x32_i8(
-                                __builtin_bit_cast(int64_t, kf[u].tail), qf[n].tail[p], c[p], 0, 0, 0);
-                    }
-                    const float f = mul[n] * ks[u];
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        // |low two| < 2^31: 256 dims of 127 * 127 times 257
-                        float v = (float)((c[NP - 2][e] << 8) + c[NP - 1][e]);
-                        if constexpr (NP == 3) v = __builtin_fmaf((float)c[0][e], 65536.0f, v);
-                        s[n][u][e] = v * f;
-                    }
-                } else {
-                    floatx4 c = {0, 0, 0, 0};
-#pragma unroll
-                    for (int p = 0; p < NP; p++)
-#pragma unroll
-                        for (int j = 0; j < O::NJ; j++)
-                            c = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[u].w[j], qf[n].w[p][j], c,
-                                                                       0, 0, 0);
-#pragma unroll
-                    for (int e = 0; e < 4; e++) s[n][u][e] = c[e] * mul[n];
+                    for (int j = 0; j < O::NJ; j++)
+                        c[p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(
+                            __builtin_bit_cast(intx4, kf[u].w[j]), qf.w[p][j], c[p], 0, 0, 0);
+                    if constexpr (O::TAIL != 0)
+                        c[p] = __builtin_amdgcn_mfma_i32_16x16x32_i8(
+                            __builtin_bit_cast(int64_t, kf[u].tail), qf.tail[p], c[p], 0, 0, 0);
                 }
+                const float f = mul * ks[u];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    // |low two| < 2^31: 256 dims of 127 * 127 times 257
+                    float v = (float)((c[NP - 2][e] << 8) + c[NP - 1][e]);
+                    if constexpr (NP == 3) v = __builtin_fmaf((float)c[0][e], 65536.0f, v);
+                    s[u][e] = v * f;
+                }
+            } else {
+                floatx4 c = {0, 0, 0, 0};
+#pragma unroll
+                for (int p = 0; p < NP; p++)
+#pragma unroll
+                    for (int j = 0; j < O::NJ; j++)
+                        c = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[u].w[j], qf.w[p][j], c, 0, 0, 0);
+#pragma unroll
+                for (int e = 0; e < 4; e++) s[u][e] = c[e] * mul;
             }
+        }
         // the next step's keys go out before this one's softmax
         if (step + kWaves < step1) {
             in++;
@@ -392,37 +422,33 @@ __global__ __launch_bounds__(256) void k_attend(KvArgs a, AttendArgs t) {
                 fetch_meta(step + kWaves);
             }
 #pragma unroll
-            for (int u = 0; u < UN; u++)
-                O::load(kf[u], a.k, place(step + kWaves, in, u), lane);
+            for (int u = 0; u < UN; u++) load(kf[u], a.k, in, u);
         }
+        bool odd = false;
         if (!whole) {
 #pragma unroll
-            for (int n = 0; n < NT; n++)
+            for (int u = 0; u < UN; u++) {
+                const int tok = step * ST + 16 * u + 4 * grp;
+                const int see = there[u] ? min(pos, x.n_tok - 1) - tok : -1;
 #pragma unroll
-                for (int u = 0; u < UN; u++)
+                for (int e = 0; e < 4; e++) s[u][e] = e <= see ? s[u][e] : -INFINITY;
+                if constexpr (!I8) {
+                    // what no row sees may be NaN, and would meet a p of zero
+                    const int n = there[u] ? min(max(x.n_tok - tok, 0), 4) : 0;
+                    const uint64_t keep = n == 4 ? ~0ull : (1ull << 16 * n) - 1;
+                    half8 z = {};
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const int tok = step * ST + 16 * u + 4 * grp + e;
-                        if (tok > pos[n] || tok >= x.n_tok || !there[u]) s[n][u][e] = -INFINITY;
+                    for (int j = 0; j < O::NJ; j++) {
+                        uintx4 w = __builtin_bit_cast(uintx4, vf[u].w[j]);
+                        w &= uintx4{(uint32_t)keep, (uint32_t)(keep >> 32), (uint32_t)keep, (uint32_t)(keep >> 32)};
+                        vf[u].w[j] = __builtin_bit_cast(half8, w);
+                        z += vf[u].w[j] * (_Float16)0.0f;
                     }
-        }
-        // values that no row may meet, and those that not every row may
-        bool odd = false;
-        if constexpr (!I8) {
-            if (!whole) {
 #pragma unroll
-                for (int u = 0; u < UN; u++)
-#pragma unroll
-                    for (int j = 0; j < O::NJ; j++)
-#pragma unroll
-                        for (int k = 0; k < 8; k++) {
-                            const int tok = step * ST + 16 * u + 4 * grp + k % 4;
-                            if (tok >= x.n_tok || !there[u]) vf[u].w[j][k] = (_Float16)0.0f;
-                            const _Float16 z = vf[u].w[j][k] * (_Float16)0.0f;
-                            odd = odd || z != z;
-                        }
-                odd = __ballot(odd) != 0;
+                    for (int k = 0; k < 8; k++) odd = odd || z[k] != z[k];
+                }
             }
+            if constexpr (!I8) odd = __ballot(odd) != 0;
         }
         float vmax = 0.0f, vmul = 0.0f, ratio[UN];
         if constexpr (I8) {
@@ -435,183 +461,151 @@ __global__ __launch_bounds__(256) void k_attend(KvArgs a, AttendArgs t) {
             for (int u = 0; u < UN; u++) ratio[u] = vs[u] * big * inv * O::kQ;
             vmul = vmax * (1.0f / O::kQ);
         }
+        float mx = -INFINITY;
 #pragma unroll
-        for (int n = 0; n < NT; n++) {
-            float mx = -INFINITY;
+        for (int u = 0; u < UN; u++)
 #pragma unroll
-            for (int u = 0; u < UN; u++)
+            for (int e = 0; e < 4; e++) mx = fmaxf(mx, s[u][e]);
+        mx = fmaxf(m, row_max(mx));
+        const float base = mx == -INFINITY ? 0.0f : mx;
+        const float keep = __builtin_amdgcn_exp2f(m - base);
+        m = mx;
+        float sum = 0.0f;
 #pragma unroll
-                for (int e = 0; e < 4; e++) mx = fmaxf(mx, s[n][u][e]);
-            mx = fmaxf(m[n], row_max(mx));
-            const float base = mx == -INFINITY ? 0.0f : mx;
-            const float keep = __builtin_amdgcn_exp2f(m[n] - base);
-            m[n] = mx;
-            float sum = 0.0f;
+        for (int u = 0; u < UN; u++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                s[u][e] = __builtin_amdgcn_exp2f(s[u][e] - (I8 ? base : base - 10.0f));
+                sum += s[u][e];
+            }
+        l = __builtin_fmaf(l, keep, sum);
+        if (__ballot(keep != 1.0f)) {
+#pragma unroll
+            for (int d = 0; d < TD; d++) acc[d] *= keep;
+        }
+        if constexpr (I8) {
+            intx4 pf[NP];
+#pragma unroll
+            for (int u = 0; u < UN; u++) {
+                uint32_t b[4], c[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++)  // the fraction's bits: p ratio, rounded
+                    b[e] = __float_as_uint(__builtin_fmaf(s[u][e], ratio[u], 8388608.0f));
+                pf[NP - 1][u] = (int)bytes4<0>(b);
+#pragma unroll
+                for (int e = 0; e < 4; e++) c[e] = b[e] + 128u;
+                pf[NP - 2][u] = (int)bytes4<1>(c);
+                if constexpr (NP == 3) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) c[e] = b[e] + 128u + 32768u;
+                    pf[0][u] = (int)bytes4<2>(c);
+                }
+            }
+#pragma unroll
+            for (int d = 0; d < TD; d++) {
+                intx4 va, c[NP];
+#pragma unroll
+                for (int u = 0; u < UN; u++)
+                    va[u] = d < 4 * O::NJ ? (int)vf[u].w[O::NJ ? d / 4 : 0][d % 4]
+                                          : (int)vf[u].tail[d % 2];
+#pragma unroll
+                for (int p = 0; p < NP; p++)
+                    c[p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(va, pf[p], intx4{0, 0, 0, 0}, 0, 0, 0);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float v = (float)((c[NP - 2][e] << 8) + c[NP - 1][e]);
+                    acc[d][e] = __builtin_fmaf(v, vmul, acc[d][e]);
+                    if constexpr (NP == 3)
+                        acc[d][e] = __builtin_fmaf((float)c[0][e], vmul * 65536.0f, acc[d][e]);
+                }
+            }
+        } else {
+            half8 pf[NP];
 #pragma unroll
             for (int u = 0; u < UN; u++)
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    s[n][u][e] = __builtin_amdgcn_exp2f(s[n][u][e] - (I8 ? base : base - 10.0f));
-                    sum += s[n][u][e];
+                    const _Float16 hi = (_Float16)s[u][e];
+                    pf[0][4 * u + e] = hi;
+                    if constexpr (NP == 2) pf[1][4 * u + e] = (_Float16)(s[u][e] - (float)hi);
                 }
-            l[n] = __builtin_fmaf(l[n], keep, sum);
-            if (__ballot(keep != 1.0f)) {
+            if (odd) {
+                // values that are not finite meet only the rows that see them,
+                // whose sums they leave NaN
+                half8 see;
 #pragma unroll
-                for (int d = 0; d < TD; d++) acc[n][d] *= keep;
-            }
-            if constexpr (I8) {
-                intx4 pf[NP];
-#pragma unroll
-                for (int u = 0; u < UN; u++) {
-                    uint32_t b[4], c[4];
-#pragma unroll
-                    for (int e = 0; e < 4; e++)  // the fraction's bits: p ratio, rounded
-                        b[e] = __float_as_uint(__builtin_fmaf(s[n][u][e], ratio[u], 8388608.0f));
-                    pf[NP - 1][u] = (int)bytes4<0>(b);
-#pragma unroll
-                    for (int e = 0; e < 4; e++) c[e] = b[e] + 128u;
-                    pf[NP - 2][u] = (int)bytes4<1>(c);
-                    if constexpr (NP == 3) {
-#pragma unroll
-                        for (int e = 0; e < 4; e++) c[e] = b[e] + 128u + 32768u;
-                        pf[0][u] = (int)bytes4<2>(c);
-                    }
-                }
+                for (int k = 0; k < 8; k++)
+                    see[k] = step * ST + 16 * (k / 4) + 4 * grp + k % 4 <= pos ? (_Float16)1.0f
+                                                                             : (_Float16)0.0f;
 #pragma unroll
                 for (int d = 0; d < TD; d++) {
-                    intx4 va, c[NP];
+                    half8 is;
 #pragma unroll
-                    for (int u = 0; u < UN; u++)
-                        va[u] = d < 4 * O::NJ ? (int)vf[u].w[O::NJ ? d / 4 : 0][d % 4]
-                                              : (int)vf[u].tail[d % 2];
-#pragma unroll
-                    for (int p = 0; p < NP; p++)
-                        c[p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(va, pf[p], intx4{0, 0, 0, 0}, 0,
-                                                                     0, 0);
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const float v = (float)((c[NP - 2][e] << 8) + c[NP - 1][e]);
-                        acc[n][d][e] = __builtin_fmaf(v, vmul, acc[n][d][e]);
-                        if constexpr (NP == 3)
-                            acc[n][d][e] = __builtin_fmaf((float)c[0][e], vmul * 65536.0f, acc[n][d][e]);
+                    for (int k = 0; k < 8; k++) {
+                        const _Float16 v = vf[k / 4].w[d / 2][4 * (d % 2) + k % 4];
+                        const _Float16 z = v * (_Float16)0.0f;
+                        is[k] = z == z ? (_Float16)0.0f : (_Float16)1.0f;
+                        if (z != z) vf[k / 4].w[d / 2][4 * (d % 2) + k % 4] = (_Float16)0.0f;
                     }
+                    const floatx4 c = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                        is, see, floatx4{0, 0, 0, 0}, 0, 0, 0);
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        if (c[e] > 0.0f) acc[d][e] = NAN;
                 }
-            } else {
-                half8 pf[NP];
+            }
+#pragma unroll
+            for (int d = 0; d < TD; d++) {
+                half8 va;
 #pragma unroll
                 for (int u = 0; u < UN; u++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const _Float16 hi = (_Float16)s[n][u][e];
-                        pf[0][4 * u + e] = hi;
-                        if constexpr (NP == 2) pf[1][4 * u + e] = (_Float16)(s[n][u][e] - (float)hi);
-                    }
+                    for (int e = 0; e < 4; e++) va[4 * u + e] = vf[u].w[d / 2][4 * (d % 2) + e];
 #pragma unroll
-                for (int d = 0; d < TD; d++) {
-                    half8 va;
-#pragma unroll
-                    for (int u = 0; u < UN; u++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++) va[4 * u + e] = vf[u].w[d / 2][4 * (d % 2) + e];
-                    if (odd) {
-                        // values that are not finite meet only the rows that
-                        // see them, whose sums they leave NaN
-                        half8 see, is;
-#pragma unroll
-                        for (int k = 0; k < 8; k++) {
-                            const int tok = step * ST + 16 * (k / 4) + 4 * grp + k % 4;
-                            const _Float16 z = va[k] * (_Float16)0.0f;
-                            is[k] = z == z ? (_Float16)0.0f : (_Float16)1.0f;
-                            va[k] = z == z ? va[k] : (_Float16)0.0f;
-                            see[k] = tok <= pos[n] ? (_Float16)1.0f : (_Float16)0.0f;
-                        }
-                        const floatx4 c = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                            is, see, floatx4{0, 0, 0, 0}, 0, 0, 0);
-#pragma unroll
-                        for (int e = 0; e < 4; e++)
-                            if (c[e] > 0.0f) acc[n][d][e] = NAN;
-                    }
-#pragma unroll
-                    for (int p = 0; p < NP; p++)
-                        acc[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pf[p], acc[n][d], 0, 0,
-                                                                           0);
-                }
+                for (int p = 0; p < NP; p++)
+                    acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pf[p], acc[d], 0, 0, 0);
             }
         }
     }
 
     // the four waves' sums, in units of 2^(their largest maximum)
-    __shared__ float s_m[kWaves][M], s_l[kWaves][M];
-    __shared__ __attribute__((aligned(16))) float s_o[kWaves / 2][M][HDP + 4];
-#pragma unroll
-    for (int n = 0; n < NT; n++) {
-        l[n] = row_sum(l[n]);
-        if (lane < 16) {
-            s_m[wave][16 * n + lane] = m[n];
-            s_l[wave][16 * n + lane] = l[n];
-        }
+    float *const s_o = reinterpret_cast<float *>(s_mem);
+    l = row_sum(l);
+    if (lane < 16) {
+        s_m[wave][lane] = m;
+        s_l[wave][lane] = l;
     }
+#pragma unroll
+    for (int d = 0; d < TD; d++)
+        *reinterpret_cast<floatx4 *>(s_o + (wave * M + (lane & 15)) * LD + 16 * d + 4 * grp) = acc[d];
     __syncthreads();
-    float top[NT];
+    const int C = (x.parts == 1 ? a.hd : HDP) / 4;
+#pragma unroll 1
+    for (int k = threadIdx.x; k < M * C; k += 256) {
+        const int i = k / C, d = 4 * (k - i * C), r = x.r0 + i;
+        if (r >= x.rows) break;
+        float top = -INFINITY, sum = 0.0f;
 #pragma unroll
-    for (int n = 0; n < NT; n++) {
-        const int r = 16 * n + (lane & 15);
-        top[n] = -INFINITY;
+        for (int w = 0; w < kWaves; w++) top = fmaxf(top, s_m[w][i]);
+        const float base = top == -INFINITY ? 0.0f : top;
+        floatx4 o = {0, 0, 0, 0};
 #pragma unroll
-        for (int w = 0; w < kWaves; w++) top[n] = fmaxf(top[n], s_m[w][r]);
-        const float base = top[n] == -INFINITY ? 0.0f : top[n];
-        const float f = __builtin_amdgcn_exp2f(m[n] - base);
-        l[n] = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kWaves; w++)
-            l[n] = __builtin_fmaf(s_l[w][r], __builtin_amdgcn_exp2f(s_m[w][r] - base), l[n]);
-#pragma unroll
-        for (int d = 0; d < TD; d++) acc[n][d] *= f;
-    }
-#pragma unroll
-    for (int from = kWaves / 2; from >= 1; from /= 2) {
-        if (wave >= from && wave < 2 * from) {
-#pragma unroll
-            for (int n = 0; n < NT; n++)
-#pragma unroll
-                for (int d = 0; d < TD; d++)
-                    *reinterpret_cast<floatx4 *>(&s_o[wave - from][16 * n + (lane & 15)][16 * d + 4 * grp]) =
-                        acc[n][d];
+        for (int w = 0; w < kWaves; w++) {
+            const float f = __builtin_amdgcn_exp2f(s_m[w][i] - base);
+            sum = __builtin_fmaf(s_l[w][i], f, sum);
+            o += *reinterpret_cast<const floatx4 *>(s_o + (w * M + i) * LD + d) * f;
         }
-        __syncthreads();
-        if (wave < from) {
-#pragma unroll
-            for (int n = 0; n < NT; n++)
-#pragma unroll
-                for (int d = 0; d < TD; d++)
-                    acc[n][d] += *reinterpret_cast<const floatx4 *>(
-                        &s_o[wave][16 * n + (lane & 15)][16 * d + 4 * grp]);
-        }
-        __syncthreads();
-    }
-    if (wave) return;
-    const int G = a.H / a.KVH;
-#pragma unroll
-    for (int n = 0; n < NT; n++) {
-        const int r = x.r0 + 16 * n + (lane & 15);
-        if (r >= x.rows) continue;
         const int64_t row = x.s.row0 + r / G;
         const int head = h * G + r % G;
         if (x.parts == 1) {
-            const float inv = l[n] == 0.0f ? 0.0f : 1.0f / l[n];
-#pragma unroll
-            for (int d = 0; d < TD; d++)
-                if (16 * d < a.hd)
-                    store4_any(a.act, t.out, row * t.ldo + (int64_t)head * a.hd + 16 * d + 4 * grp,
-                               t.vec, acc[n][d] * inv);
+            store4_any(a.act, t.out, row * t.ldo + (int64_t)head * a.hd + d, t.vec,
+                       o * (sum == 0.0f ? 0.0f : 1.0f / sum));
         } else {
             const int64_t at = (row * a.H + head) * t.splits + split;
-#pragma unroll
-            for (int d = 0; d < TD; d++)
-                *reinterpret_cast<floatx4 *>(t.part_o + at * HDP + 16 * d + 4 * grp) = acc[n][d];
-            if (lane < 16) {
-                t.part_ml[2 * at] = top[n];
-                t.part_ml[2 * at + 1] = l[n];
+            *reinterpret_cast<floatx4 *>(t.part_o + at * HDP + d) = o;
+            if (d == 0) {
+                t.part_ml[2 * at] = top;
+                t.part_ml[2 * at + 1] = sum;
             }
         }
     }
@@ -664,13 +658,13 @@ __global__ __launch_bounds__(256) void k_attend_join(KvArgs a, AttendArgs t) {
                o * (l == 0.0f ? 0.0f : 1.0f / l));
 }
 
-// Launches over `tiles` tiles: of 16 rows (attend_*), or of 32 W rows, W waves
-// (prompt_*), with the join where blocks share rows.
+// Launches over `tiles` tiles: of 16 rows (attend_*), or of many (kManyRows * 32)
+// or 64 rows (prompt_*), with the join where blocks share rows.
 hipError_t attend_i8(const KvArgs &a, const AttendArgs &t, int tiles, hipStream_t st);
 hipError_t attend_f16(const KvArgs &a, const AttendArgs &t, int tiles, hipStream_t st);
-hipError_t prompt_f32(const KvArgs &a, const AttendArgs &t, int tiles, int waves, hipStream_t st);
-hipError_t prompt_f16(const KvArgs &a, const AttendArgs &t, int tiles, int waves, hipStream_t st);
-hipError_t prompt_bf16(const KvArgs &a, const AttendArgs &t, int tiles, int waves, hipStream_t st);
+hipError_t prompt_f32(const KvArgs &a, const AttendArgs &t, int tiles, bool many, hipStream_t st);
+hipError_t prompt_f16(const KvArgs &a, const AttendArgs &t, int tiles, bool many, hipStream_t st);
+hipError_t prompt_bf16(const KvArgs &a, const AttendArgs &t, int tiles, bool many, hipStream_t st);
 
 template <int ST, int M, int LEAST>
 hipError_t attend_join(const KvArgs &a, const AttendArgs &t, int tiles, hipStream_t st) {
@@ -696,7 +690,7 @@ void by_dims(const KvArgs &a, F f) {
 template <bool I8, int NP>
 hipError_t attend_launch(const KvArgs &a, const AttendArgs &t, int tiles, hipStream_t st) {
     by_dims(a, [&](auto ns) {
-        hipLaunchKernelGGL((k_attend<I8, NP, decltype(ns)::value, 1>),
+        hipLaunchKernelGGL((k_attend<I8, NP, decltype(ns)::value>),
                            dim3((unsigned)tiles * a.KVH, t.splits), dim3(256), 0, st, a, t);
     });
     return attend_join<kStep<I8>, 16, kWaves>(a, t, tiles, st);

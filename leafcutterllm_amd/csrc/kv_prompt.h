@@ -49,225 +49,249 @@ __device__ __forceinline__ float pair_sum(float v) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// groups of 32 rows of a block of many, and shares of the context of one of 64
+// rows: as many as the registers of a head allow
+template <int NS> constexpr int kManyRows = NS <= 4 ? 8 : 4;
+template <int NS> constexpr int kShares = NS <= 4 ? 4 : 2;
 // steps that a block is worth, where blocks share rows
-constexpr int kPromptLeast = 2;
+template <int WT> constexpr int kPromptLeast = 2 * WT;
 // m of a row that has met no key
 constexpr float kNone = -1e30f;
 template <int ACT> constexpr int kQPieces = ACT == LCMOE_TYPE_BF16 ? 1 : 2;
 template <int ACT> constexpr int kPPieces = ACT == LCMOE_TYPE_F32 ? 2 : 1;
 
-// A step's keys and values between global memory and LDS.  A thread moves
-// items of two chunks of a 16-token unit, its lane's: lane = unit * 16 + r.
-// Keys (r: token): the two 8-dim halves of 16 dims.  Values (r: dim): tokens
-// 4 g .. + 3 and 8 + 4 g .. + 3 of 2 (narrow) or 4 (wide) dims 16 apart.
+// What a load has brought, copied here: the compiler would copy it to the next
+// turn's register at the end of the loop, and wait for the load there.
+template <class T>
+__device__ __forceinline__ T arrived(T x) {
+    T y;
+    asm volatile("v_mov_b32 %0, %1" : "=v"(y) : "v"(x));
+    return y;
+}
+
+// A step's keys and values between global memory and LDS.  A lane moves items
+// of two chunks of its 16-token unit: lane = unit * 16 + r.  Keys (r: token):
+// two neighbouring groups of dims, so that an item is 32 (wide) or 16 (narrow)
+// dims.  Values (r: dim): token groups g and g + 2, of 4 (wide) or 2 (narrow)
+// dims 16 apart.  A wave's items are known by its number alone, and every one
+// is the same two loads, so that nothing waits for a load but its store.
 template <bool I8, int NS, int W>
 struct Staged {
     static constexpr int NJ = I8 ? NS / 2 : 0, NB = I8 ? NS & 1 : NS;  // wide, narrow blocks
-    // items per lane set of 64: keys 4 (wide) or 2 (narrow) of 16 dims a
-    // block, values 2 of the two token groups
-    static constexpr int KW = 4 * NJ, VW = 2 * NJ, KN = 2 * NB, VN = 2 * NB;
-    static constexpr int IT = KW + VW + KN + VN, PER = (IT + W - 1) / W;
-    // a wide key item is one 16-byte chunk, a wide value item two; a narrow
-    // item two chunks of 8 (8 bits) or 16 bytes
-    uintx4 x[PER][2];
+    // items: of each block two of keys, then two of values
+    static constexpr int WI = 4 * NJ, NI = 4 * NB;
+    static constexpr int PW = (WI + W - 1) / W, PN = (NI + W - 1) / W;
+    uintx4 x[PW ? PW : 1][2], y[PN ? PN : 1][2];  // narrow 8-bit chunks: 8 bytes each, in y[.][0]
 
     __device__ __forceinline__ void load(const KvArgs &a, int wave, int lane, int page, int h,
                                          int unit) {
         const int r = lane & 15;
-        const int64_t at = unit_base(a, page, h, unit);
+        const int64_t at = unit_base(a, page, h, unit) * (I8 ? 1 : 2);
 #pragma unroll
-        for (int k = 0; k < PER; k++) {
-            int i = wave + k * W;
-            if (i >= IT) break;
-            if (I8 && i < KW) {
-                x[k][0] = *reinterpret_cast<const uintx4 *>(a.k + at + (i >> 2) * 1024 + (i & 3) * 256 + r * 16);
-            } else if (I8 && i < KW + VW) {
-                i -= KW;
-                const uint8_t *p = a.v + at + (i >> 1) * 1024 + (i & 1) * 256 + r * 16;
-                x[k][0] = *reinterpret_cast<const uintx4 *>(p);
-                x[k][1] = *reinterpret_cast<const uintx4 *>(p + 512);
+        for (int k = 0; k < PW; k++) {
+            const int i = min(wave + k * W, WI - 1);
+            const bool value = i >= 2 * NJ;
+            const int j = value ? i - 2 * NJ : i;
+            const uint8_t *p = (value ? a.v : a.k) + at + (j >> 1) * 1024 + r * 16;
+            x[k][0] = *reinterpret_cast<const uintx4 *>(p + (value ? 256 : 512) * (j & 1));
+            x[k][1] = *reinterpret_cast<const uintx4 *>(p + (value ? 256 : 512) * (j & 1) + (value ? 512 : 256));
+        }
+        constexpr int C = I8 ? 8 : 16;  // bytes of a chunk
+#pragma unroll
+        for (int k = 0; k < PN; k++) {
+            const int i = min(wave + k * W, NI - 1);
+            const bool value = i >= 2 * NB;
+            const int j = value ? i - 2 * NB : i;
+            const uint8_t *p = (value ? a.v : a.k) + at + NJ * 1024 + (j >> 1) * 64 * C + r * C +
+                               (value ? 16 : 32) * C * (j & 1);
+            const int next = (value ? 32 : 16) * C;
+            if constexpr (I8) {
+                const uintx2 u = *reinterpret_cast<const uintx2 *>(p);
+                const uintx2 v = *reinterpret_cast<const uintx2 *>(p + next);
+                y[k][0] = uintx4{u[0], u[1], v[0], v[1]};
             } else {
-                i -= KW + VW;
-                const bool value = i >= KN;
-                if (value) i -= KN;
-                const uint8_t *pool = value ? a.v : a.k;
-                // keys: groups 2 s, 2 s + 1; values: g, g + 2
-                const int g0 = value ? i & 1 : 2 * (i & 1), g1 = value ? g0 + 2 : g0 + 1;
-                if constexpr (I8) {
-                    const uint8_t *p = pool + at + NJ * 1024 + r * 8;
-                    const uintx2 u = *reinterpret_cast<const uintx2 *>(p + g0 * 128);
-                    const uintx2 v = *reinterpret_cast<const uintx2 *>(p + g1 * 128);
-                    x[k][0] = uintx4{u[0], u[1], v[0], v[1]};
-                } else {
-                    const uint8_t *p = pool + 2 * at + (i >> 1) * 1024 + r * 16;
-                    x[k][0] = *reinterpret_cast<const uintx4 *>(p + g0 * 256);
-                    x[k][1] = *reinterpret_cast<const uintx4 *>(p + g1 * 256);
-                }
+                y[k][0] = *reinterpret_cast<const uintx4 *>(p);
+                y[k][1] = *reinterpret_cast<const uintx4 *>(p + next);
             }
         }
     }
 
     // sk [2 tiles of 32 tokens][2 NS sets of 16 dims][2][32 tokens][8 dims]
-    // sv [4 units][NS][2][32 dims][8 tokens]; there: whether the lane's page is
-    // Returns whether a value is not finite (f16, and only where `edge` asks).
+    // sv [4 units][NS][2][32 dims][8 tokens]; there: whether the lane's page is.
+    // f16, where `edge` asks: a value that is not finite is stored as zero, and
+    // its token's bit set in bad[dim]; returns whether there is one.
     __device__ __forceinline__ bool store(half8 *sk, half8 *sv, int wave, int lane, int tokens,
-                                          bool there, bool edge) const {
+                                          bool there, bool edge, unsigned long long *bad) const {
         bool odd = false;
         const int unit = lane >> 4, r = lane & 15;
         half8 *kd = sk + (unit >> 1) * (2 * NS) * 64 + (unit & 1) * 16 + r;
-        half8 *vd = sv + unit * NS * 64;
+        half8 *vd = sv + unit * NS * 64 + r;
 #pragma unroll
-        for (int k = 0; k < PER; k++) {
-            int i = wave + k * W;
-            if (i >= IT) break;
-            if (I8 && i < KW) {
-                kd[i * 64] = cat(codes4(x[k][0][0]), codes4(x[k][0][1]));
-                kd[i * 64 + 32] = cat(codes4(x[k][0][2]), codes4(x[k][0][3]));
-            } else if (I8 && i < KW + VW) {
-                i -= KW;
+        for (int k = 0; k < PW; k++) {
+            const int i = wave + k * W, j = i >= 2 * NJ ? i - 2 * NJ : i;
+            if (i < 2 * NJ) {  // dims 64 (j / 2) + 32 (j % 2): sets 2 j, 2 j + 1
+#pragma unroll
+                for (int c = 0; c < 2; c++)
+#pragma unroll
+                    for (int g = 0; g < 2; g++)
+                        kd[(2 * j + c) * 64 + g * 32] =
+                            cat(codes4(x[k][c][2 * g]), codes4(x[k][c][2 * g + 1]));
+            } else if (i < WI) {
 #pragma unroll
                 for (int t = 0; t < 4; t++)
-                    vd[(2 * (i >> 1) + (t >> 1)) * 64 + (i & 1) * 32 + (t & 1) * 16 + r] =
+                    vd[(2 * (j >> 1) + (t >> 1)) * 64 + (j & 1) * 32 + (t & 1) * 16] =
                         cat(codes4(x[k][0][t]), codes4(x[k][1][t]));
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < PN; k++) {
+            const int i = wave + k * W;
+            if (i >= NI) break;
+            half4 c[4];  // chunk 0, chunk 1: of 8 dims, or of 2 dims by 4 tokens
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+                c[t] = I8 ? codes4(y[k][0][t])
+                          : __builtin_bit_cast(half4, uintx2{y[k][t >> 1][2 * (t & 1)],
+                                                             y[k][t >> 1][2 * (t & 1) + 1]});
+            if (i < 2 * NB) {
+                kd[(4 * NJ + i) * 64] = cat(c[0], c[1]);
+                kd[(4 * NJ + i) * 64 + 32] = cat(c[2], c[3]);
             } else {
-                i -= KW + VW;
-                const bool value = i >= KN;
-                if (value) i -= KN;
-                half4 c[4];
-                if constexpr (I8) {
+                const int j = i - 2 * NB, g = j & 1, b = 2 * NJ + (j >> 1);
+                if constexpr (!I8) {
+                    // what is behind the last token, or not there, may be NaN:
+                    // it would meet a p of zero
+                    if (!there || tokens < 64) {
 #pragma unroll
-                    for (int t = 0; t < 4; t++) c[t] = codes4(x[k][0][t]);
-                } else {
+                        for (int h = 0; h < 2; h++) {
+                            const int n = there ? min(max(tokens - unit * 16 - 8 * h - 4 * g, 0), 4) : 0;
+                            const uint64_t keep = n == 4 ? ~0ull : (1ull << 16 * n) - 1;
 #pragma unroll
-                    for (int t = 0; t < 4; t++)
-                        c[t] = __builtin_bit_cast(half4, uintx2{x[k][t >> 1][2 * (t & 1)],
-                                                                x[k][t >> 1][2 * (t & 1) + 1]});
-                }
-                const int b = 2 * NJ + (i >> 1);  // 32 dims
-                if (!value) {
-                    kd[(2 * b + (i & 1)) * 64] = cat(c[0], c[1]);
-                    kd[(2 * b + (i & 1)) * 64 + 32] = cat(c[2], c[3]);
-                } else {
-                    const int g = i & 1;
-                    if constexpr (!I8) {
-                        // what is behind the last token, or not there, may be
-                        // NaN: it would meet a p of zero
-                        if (!there || tokens < 64) {
-#pragma unroll
-                            for (int t = 0; t < 4; t++)
-#pragma unroll
-                                for (int e = 0; e < 4; e++)
-                                    if (!there || unit * 16 + 8 * (t >> 1) + 4 * g + e >= tokens)
-                                        c[t][e] = (_Float16)0.0f;
+                            for (int t = 2 * h; t < 2 * h + 2; t++)
+                                c[t] = __builtin_bit_cast(half4, __builtin_bit_cast(uint64_t, c[t]) & keep);
                         }
                     }
-                    if (!I8 && edge) {
-                        const half4 z = c[0] * (_Float16)0.0f + c[1] * (_Float16)0.0f +
-                                        c[2] * (_Float16)0.0f + c[3] * (_Float16)0.0f;
+                    const half4 z = (c[0] + c[1] + c[2] + c[3]) * (_Float16)0.0f;
+                    if (edge && __builtin_expect(
+                                    __ballot(z[0] + z[1] + z[2] + z[3] != (_Float16)0.0f) != 0, 0)) {
 #pragma unroll
-                        for (int e = 0; e < 4; e++) odd = odd || z[e] != z[e];
+                        for (int t = 0; t < 4; t++) {
+                            unsigned long long bits = 0;
+#pragma unroll
+                            for (int e = 0; e < 4; e++) {
+                                const _Float16 z = c[t][e] * (_Float16)0.0f;
+                                if (z == z) continue;
+                                c[t][e] = (_Float16)0.0f;
+                                bits |= 1ull << (unit * 16 + 8 * (t >> 1) + 4 * g + e);
+                            }
+                            if (bits) {
+                                atomicOr(&bad[32 * b + 16 * (t & 1) + r], bits);
+                                odd = true;
+                            }
+                        }
                     }
-                    vd[b * 64 + g * 32 + r] = cat(c[0], c[2]);
-                    vd[b * 64 + g * 32 + 16 + r] = cat(c[1], c[3]);
                 }
+                vd[b * 64 + g * 32] = cat(c[0], c[2]);
+                vd[b * 64 + g * 32 + 16] = cat(c[1], c[3]);
             }
         }
         return odd;
     }
 };
 
-template <int ACT, bool I8, int NS, int W>
-__global__ __launch_bounds__(64 * W, W == 8 ? 2 : 1) void k_attend_prompt(KvArgs a, AttendArgs t) {
-    constexpr int NQ = kQPieces<ACT>, NP = kPPieces<ACT>, KS = 2 * NS;
-    constexpr float kLog2e = 1.44269504088896340736f;
-    __shared__ __attribute__((aligned(16))) half8 s_k[2][2 * KS * 64], s_v[2][4 * NS * 64];
+// The order of the instructions around it: LDS reads run four operands ahead
+// of the `per` matrix instructions that take one.
+template <int READS, int PER>
+__device__ __forceinline__ void read_ahead() {
+    constexpr int A = READS < 4 ? READS : 4;
+    __builtin_amdgcn_sched_group_barrier(0x100, A, 0);
+#pragma unroll
+    for (int i = 0; i < READS; i++) {
+        __builtin_amdgcn_sched_group_barrier(0x008, PER, 0);
+        if (i + A < READS) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+}
+
+// WR WT waves: WR groups of 32 rows, WT shares of the context, which take the
+// block's steps in turn, each with buffers of its own, and add up at the end.
+// WT = 1: two buffers, so that a step is brought in beside the one before.
+template <int ACT, bool I8, int NS, int WR, int WT>
+__global__ __launch_bounds__(64 * WR * WT, NS <= 4 ? 2 : 1) void k_attend_prompt(KvArgs a, AttendArgs t) {
+    constexpr int NQ = kQPieces<ACT>, NP = kPPieces<ACT>, KS = 2 * NS, M = 32 * WR;
+    constexpr int KB = 2 * KS * 64, VB = 4 * NS * 64, BUFS = WT == 1 ? 2 : WT;
+    constexpr int QB = WR * NQ * KS * 64;
+    __shared__ __attribute__((aligned(16))) half8 s_kv[BUFS * (KB + VB) > QB ? BUFS * (KB + VB) : QB];
+    __shared__ float s_mul[M];
+    // f16 pages: of a step that not every row of the block sees, the tokens
+    // whose values are not finite, by dim; by turn, and whether there are any
+    __shared__ unsigned long long s_bad[I8 ? 1 : WT * 4][I8 ? 1 : 32 * NS];
+    __shared__ int s_odd[WT][4];
+    half8 *const s_k = s_kv, *const s_v = s_kv + BUFS * KB;
     const int lane = threadIdx.x & 63, row = lane & 31, g = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wr = wave % WR, wt = wave / WR;
     const int h = blockIdx.x % a.KVH, split = blockIdx.y, G = a.H / a.KVH;
     Tile x;
-    if (!find_rows<64, 32 * W, kPromptLeast>(a, t, gridDim.x / a.KVH - 1 - blockIdx.x / a.KVH, x)) return;
+    if (!find_rows<64, M, kPromptLeast<WT>>(a, t, gridDim.x / a.KVH - 1 - blockIdx.x / a.KVH, x)) return;
     if (split >= x.parts) return;
-    const int step0 = split * x.per, step1 = min(x.steps, (split + 1) * x.per);
+    const int step0 = split * x.per + wt, step1 = min(x.steps, (split + 1) * x.per);
+    const int turns = (step1 - split * x.per + WT - 1) / WT;
 
     // pages: the lane's unit of the step that is being brought in
     const int32_t *table = a.pages + (int64_t)x.b * a.max_pages;
     const int ushift = a.plog - 4, last_unit = (x.n_tok - 1) >> 4;
     const auto page_of = [&](int step) {
-        const int p = table[min(step * 4 + (lane >> 4), last_unit) >> ushift];
-        return p < a.n_pages ? p : -1;
+        return table[min(step * 4 + (lane >> 4), last_unit) >> ushift];
     };
-    const auto unit_of = [&](int step) {
-        return min(step * 4 + (lane >> 4), last_unit) & ((1 << ushift) - 1);
-    };
-    Staged<I8, NS, W> st;
+    const auto is_there = [&](int p) { return p >= 0 && p < a.n_pages; };
+    Staged<I8, NS, WR> st;
     float sks = 0.0f, svs = 0.0f;  // scales of the lane's unit, of the step being brought in
     int page = page_of(step0);
     const auto bring = [&](int step) {
-        st.load(a, wave, lane, max(page, 0), h, unit_of(step));
+        const int p = is_there(page) ? page : 0;
+        st.load(a, wr, lane, p, h, min(step * 4 + (lane >> 4), last_unit) & ((1 << ushift) - 1));
         if constexpr (I8) {
-            const float *s = a.scale + ((int64_t)max(page, 0) * a.KVH + h) * 2;
+            const float *s = a.scale + ((int64_t)p * a.KVH + h) * 2;
             sks = s[0];
             svs = s[1];
         }
     };
     bring(step0);
+    int page_ahead = page_of(step0 + WT);
 
     // the wave's rows
-    const int r = x.r0 + 32 * wave + row, i = r / G;
+    const int first = x.r0 + 32 * wr, r = first + row, i = r / G;
     const bool valid = r < x.rows;
     const int pos = valid ? x.s.len0 + i : 0x7fffffff;
-    const int r_last = min(x.r0 + 32 * wave + 31, x.rows - 1);
-    const bool any = x.r0 + 32 * wave < x.rows;
-    const int all_see = x.s.len0 + (x.r0 + 32 * wave) / G + 1;
-    const int n_tok = any ? x.s.len0 + r_last / G + 1 : 0;
-    half8 qf[NQ][KS];
-    float mul;
-    {
-        const int half = a.hd / 2;
-        const int64_t e = (int64_t)(x.s.row0 + i) * t.ldq + (int64_t)(h * G + r % G) * a.hd;
-        const float *cs = t.rope + (int64_t)(a.rope_abs ? x.s.len0 + i : i) * a.hd;
-        float y[KS][8], most = 0.0f, bad = 0.0f;
-#pragma unroll
-        for (int c = 0; c < KS; c++) {
-            const int d = 16 * c + 8 * g;
-            if (valid && d < a.hd) {
-                load8<ACT>(t.q, e + d, t.vec, y[c]);
-                if (t.rope) {
-                    const bool up = d >= half;
-                    const int o = up ? d - half : d;
-                    float z[8];
-                    load8<ACT>(t.q, e + (up ? o : d + half), t.vec, z);
-                    const float *w = cs + 2 * o;
-#pragma unroll
-                    for (int k = 0; k < 8; k++)
-                        y[c][k] = up ? z[k] * w[2 * k + 1] + y[c][k] * w[2 * k]
-                                     : y[c][k] * w[2 * k] - z[k] * w[2 * k + 1];
-                }
-            } else {
-#pragma unroll
-                for (int k = 0; k < 8; k++) y[c][k] = 0.0f;
-            }
-#pragma unroll
-            for (int k = 0; k < 8; k++) {
-                most = fmaxf(most, fabsf(y[c][k]));
-                bad = __builtin_fmaf(y[c][k], 0.0f, bad);  // NaN where y is not finite
-            }
-        }
-        most = pair_max(most);
-        bad = pair_sum(bad);
-        // the row's largest to [2^14, 2^15): pieces are normal f16 values
-        const int ex = most > 0.0f && most < INFINITY ? __builtin_amdgcn_frexp_expf(most) : 0;
-        mul = __builtin_amdgcn_ldexpf(t.scale, ex - 15) * kLog2e + bad;
-#pragma unroll
-        for (int c = 0; c < KS; c++)
-#pragma unroll
-            for (int k = 0; k < 8; k++) {
-                const float v = __builtin_amdgcn_ldexpf(y[c][k], 15 - ex);
-                const _Float16 hi = (_Float16)v;
-                qf[0][c][k] = hi;
-                if constexpr (NQ == 2) qf[1][c][k] = (_Float16)(v - (float)hi);
-            }
+    const int all_see = x.s.len0 + first / G + 1;
+    const int n_tok = first < x.rows ? x.s.len0 + min(first + 31, x.rows - 1) / G + 1 : 0;
+    if constexpr (!I8) {
+#pragma unroll 1
+        for (int k = threadIdx.x; k < WT * 4 * 32 * NS; k += 64 * WR * WT) (&s_bad[0][0])[k] = 0;
+        if (threadIdx.x < 4 * WT) (&s_odd[0][0])[threadIdx.x] = 0;
     }
+    // its operands, through LDS: [group of rows][piece][16 dims][lane]
+    half8 *const s_q = s_kv;
+    stage_q<NS, M, 64 * WR * WT>(a, t, x, h,
+        [&](int64_t e, float (&y)[8]) { load8<ACT>(t.q, e, t.vec, y); },
+        [&](int r, int c, const float (&y)[8], float most) {
+            half8 o[NQ];
+            half_pieces<NQ>(y, exponent_of(most), o);
+#pragma unroll
+            for (int p = 0; p < NQ; p++)
+                s_q[(((r >> 5) * NQ + p) * KS + (c >> 1)) * 64 + (c & 1) * 32 + (r & 31)] = o[p];
+        },
+        [&](int r, float most, float bad) {
+            s_mul[r] = __builtin_amdgcn_ldexpf(t.scale, exponent_of(most) - 15) * kLog2e + bad;
+        });
+    __syncthreads();
+    half8 qf[NQ][KS];
+#pragma unroll
+    for (int p = 0; p < NQ; p++)
+#pragma unroll
+        for (int c = 0; c < KS; c++) qf[p][c] = s_q[((wr * NQ + p) * KS + c) * 64 + lane];
+    const float mul = s_mul[32 * wr + row];
+    __syncthreads();  // the buffers are the steps' from here on
 
     floatx16 acc[NS];
 #pragma unroll
@@ -275,22 +299,50 @@ __global__ __launch_bounds__(64 * W, W == 8 ? 2 : 1) void k_attend_prompt(KvArgs
 #pragma unroll
         for (int e = 0; e < 16; e++) acc[d][e] = 0.0f;
     // m: below every score at first; l: 2^6 sum of 2^(S - m), the lane's share
-    float m = kNone, l = 0.0f, U = 0.0f;
-    int buf = 0;
-    // whether some row of the block does not see all of a step
-    const auto edge_of = [&](int step) { return (step + 1) * 64 > x.all_see; };
-    bool odd = st.store(s_k[0], s_v[0], wave, lane, x.n_tok - step0 * 64, page >= 0, edge_of(step0));
+    float m = kNone, l = 0.0f, U = 0.0f, log_U = 0.0f;
     int there = page;
     float ks_now = sks, vs_now = svs;
-    page = page_of(min(step0 + 1, x.steps - 1));
-    // the step's barrier; where it matters, odd becomes the block's
-    const auto meet = [&](bool edge) {
-        if (!I8 && edge) odd = __syncthreads_or(odd);
-        else __syncthreads();
+    // whether some row of the block does not see all of a step
+    const auto edge_of = [&](int step) { return (step + 1) * 64 > x.all_see; };
+    const auto store = [&](int step, int n, int buf) {
+        unsigned long long *const bad = s_bad[I8 ? 0 : wt * 4 + (n & 3)];
+        const bool odd = st.store(s_k + buf * KB, s_v + buf * VB, wr, lane, x.n_tok - step * 64,
+                                  is_there(page), edge_of(step), bad);
+        if constexpr (!I8) {
+            if (odd) s_odd[wt][n & 3] = 1;
+            // the turn after the next: its last reader passed a barrier ago
+            if (edge_of(step + 2 * WT)) {
+                if (wr == 0 && lane == 0) s_odd[wt][(n + 2) & 3] = 0;
+                for (int k = wr * 64 + lane; k < 32 * NS; k += 64 * WR)
+                    s_bad[wt * 4 + ((n + 2) & 3)][k] = 0;
+            }
+        }
     };
-    meet(edge_of(step0));
-    for (int step = step0; step < step1; step++) {
-        const uint64_t have = __ballot(there >= 0);
+    // what has arrived becomes the step's, and the next one is sent for; past
+    // the last it is again: a branch would make the loads' registers wait
+    const auto send = [&](int step) {
+        there = page;
+        if constexpr (I8) {
+            ks_now = arrived(sks);
+            vs_now = arrived(svs);
+        }
+        page = arrived(page_ahead);
+        bring(step);
+        page_ahead = page_of(step + WT);
+    };
+    if constexpr (WT == 1) {
+        store(step0, 0, 0);
+        __syncthreads();
+        send(step0 + 1);
+    }
+    for (int n = 0; n < turns; n++) {
+        const int step = step0 + n * WT, buf = WT == 1 ? n & 1 : wt;
+        if constexpr (WT > 1) {
+            store(step, n, buf);
+            __syncthreads();
+            send(step + WT);
+        }
+        const uint64_t have = __ballot(is_there(there));
         bool missing = false;
         float ks[4], vs[4];
 #pragma unroll
@@ -302,28 +354,27 @@ __global__ __launch_bounds__(64 * W, W == 8 ? 2 : 1) void k_attend_prompt(KvArgs
                 if (!(have >> (16 * u) & 1)) ks[u] = vs[u] = 0.0f;
             }
         }
-        const bool more = step + 1 < step1;
-        int next_page = 0;
-        if (more) {
-            bring(step + 1);
-            next_page = page_of(min(step + 2, x.steps - 1));
-        }
-        if (step * 64 < n_tok) {
+        if (step < step1 && step * 64 < n_tok) {
+            const bool whole = !missing && (step + 1) * 64 <= all_see;
+            const half8 *const kp = s_k + buf * KB + lane, *const vp = s_v + buf * VB + lane;
             floatx16 c[2];
 #pragma unroll
             for (int tt = 0; tt < 2; tt++)
 #pragma unroll
                 for (int e = 0; e < 16; e++) c[tt][e] = 0.0f;
+            // a product on the same sums waits for the one before: turn by turn
 #pragma unroll
-            for (int s = 0; s < KS; s++)
+            for (int s = 0; s < KS; s++) {
+                half8 ka[2];
 #pragma unroll
-                for (int tt = 0; tt < 2; tt++) {
-                    const half8 ka = s_k[buf][(tt * KS + s) * 64 + lane];
+                for (int tt = 0; tt < 2; tt++) ka[tt] = kp[(tt * KS + s) * 64];
 #pragma unroll
-                    for (int p = 0; p < NQ; p++)
-                        c[tt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka, qf[p][s], c[tt], 0, 0, 0);
-                }
-            const bool whole = !missing && (step + 1) * 64 <= all_see;
+                for (int p = 0; p < NQ; p++)
+#pragma unroll
+                    for (int tt = 0; tt < 2; tt++)
+                        c[tt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka[tt], qf[p][s], c[tt], 0, 0, 0);
+            }
+            read_ahead<2 * KS, NQ>();
             // exponents' factors and offsets by unit; l's weights
             float f[4], off[4], weight[4];
             if constexpr (I8) {
@@ -333,15 +384,18 @@ __global__ __launch_bounds__(64 * W, W == 8 ? 2 : 1) void k_attend_prompt(KvArgs
 #pragma unroll
                     for (int d = 0; d < NS; d++) acc[d] *= k;
                     U = vmax;
+                    log_U = __builtin_amdgcn_logf(U);
                 }
 #pragma unroll
                 for (int u = 0; u < 4; u++) {
                     // codes of a page without values are zeros, in any scale;
                     // under 2^-60 of U none of them is left in f16
-                    const float w = vs[u] > 0.0f ? fmaxf(vs[u] / U, 0x1p-60f) : 1.0f;
+                    const float w = vs[u] > 0.0f
+                                        ? fmaxf(__builtin_amdgcn_logf(vs[u]) - log_U, -60.0f)
+                                        : 0.0f;
                     f[u] = mul * ks[u];
-                    off[u] = 6.0f + __builtin_amdgcn_logf(w);
-                    weight[u] = 1.0f / w;
+                    off[u] = 6.0f + w;
+                    weight[u] = __builtin_amdgcn_exp2f(-w);
                 }
             } else {
 #pragma unroll
@@ -366,12 +420,12 @@ __global__ __launch_bounds__(64 * W, W == 8 ? 2 : 1) void k_attend_prompt(KvArgs
                     c[tt][e] = __builtin_fmaf(c[tt][e], f[2 * tt + e / 8], base[2 * tt + e / 8]);
             if (!whole) {
 #pragma unroll
-                for (int tt = 0; tt < 2; tt++)
+                for (int u = 0; u < 4; u++) {
+                    const int see = have >> (16 * u) & 1 ? pos - (step * 64 + 16 * u + 4 * g) : -1;
 #pragma unroll
-                    for (int e = 0; e < 16; e++) {
-                        const int tok = step * 64 + 32 * tt + 8 * (e / 4) + 4 * g + e % 4;
-                        if (tok > pos || !(have >> (16 * (2 * tt + e / 8)) & 1)) c[tt][e] = -INFINITY;
-                    }
+                    for (int e = 0; e < 8; e++)
+                        if (8 * (e / 4) + e % 4 > see) c[u / 2][8 * (u & 1) + e] = -INFINITY;
+                }
             }
 #pragma unroll
             for (int tt = 0; tt < 2; tt++)
@@ -413,84 +467,117 @@ __global__ __launch_bounds__(64 * W, W == 8 ? 2 : 1) void k_attend_prompt(KvArgs
                     }
                     l = __builtin_fmaf(sum, weight[2 * tt + j], l);
                 }
-            if (I8 || !odd || whole) {
 #pragma unroll
-                for (int u = 0; u < 4; u++)
+            for (int u = 0; u < 4; u++) {
+                half8 va[NS];
 #pragma unroll
-                    for (int d = 0; d < NS; d++) {
-                        const half8 va = s_v[buf][(u * NS + d) * 64 + lane];
+                for (int d = 0; d < NS; d++) va[d] = vp[(u * NS + d) * 64];
 #pragma unroll
-                        for (int p = 0; p < NP; p++)
-                            acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, pf[p][u], acc[d], 0, 0, 0);
-                    }
-            } else {
-                // values that are not finite meet only the rows that see them,
-                // whose sums they leave NaN
-#pragma unroll 1
-                for (int u = 0; u < 4; u++) {
-                    half8 see, pu[NP];
+                for (int p = 0; p < NP; p++)
 #pragma unroll
-                    for (int k = 0; k < 8; k++) {
-                        const int tok = step * 64 + 16 * u + 8 * (k / 4) + 4 * g + k % 4;
-                        see[k] = tok <= pos ? (_Float16)1.0f : (_Float16)0.0f;
-                    }
+                    for (int d = 0; d < NS; d++)
+                        acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va[d], pf[p][u], acc[d], 0, 0, 0);
+            }
+            read_ahead<4 * NS, NP>();
+            if constexpr (!I8) {
+                if (s_odd[wt][n & 3]) {
+                    // the rows that see a token whose value is not finite
+                    const int last = min(pos - step * 64, 63);
+                    const unsigned long long see = last < 0 ? 0 : ~0ull >> (63 - last);
 #pragma unroll
-                    for (int p = 0; p < NP; p++)
-                        pu[p] = u == 0 ? pf[p][0] : u == 1 ? pf[p][1] : u == 2 ? pf[p][2] : pf[p][3];
-#pragma unroll
-                    for (int d = 0; d < NS; d++) {
-                        half8 va = s_v[buf][(u * NS + d) * 64 + lane], is;
-#pragma unroll
-                        for (int k = 0; k < 8; k++) {
-                            const _Float16 z = va[k] * (_Float16)0.0f;
-                            is[k] = z == z ? (_Float16)0.0f : (_Float16)1.0f;
-                            va[k] = z == z ? va[k] : (_Float16)0.0f;
-                        }
-                        floatx16 seen;
-#pragma unroll
-                        for (int e = 0; e < 16; e++) seen[e] = 0.0f;
-                        seen = __builtin_amdgcn_mfma_f32_32x32x16_f16(is, see, seen, 0, 0, 0);
+                    for (int d = 0; d < NS; d++)
 #pragma unroll
                         for (int e = 0; e < 16; e++)
-                            if (seen[e] > 0.0f) acc[d][e] = NAN;
-#pragma unroll
-                        for (int p = 0; p < NP; p++)
-                            acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, pu[p], acc[d], 0, 0, 0);
-                        __builtin_amdgcn_sched_barrier(0);  // one at a time: few registers
-                    }
+                            if (s_bad[wt * 4 + (n & 3)][32 * d + 8 * (e / 4) + 4 * g + e % 4] & see)
+                                acc[d][e] = NAN;
                 }
             }
         }
-        if (more) {
-            odd = st.store(s_k[buf ^ 1], s_v[buf ^ 1], wave, lane, x.n_tok - (step + 1) * 64, page >= 0,
-                           edge_of(step + 1));
-            there = page;
-            ks_now = sks;
-            vs_now = svs;
-            page = next_page;
+        if constexpr (WT == 1) {
+            if (n + 1 < turns) store(step + 1, n + 1, buf ^ 1);
+            __syncthreads();
+            send(step + 2);
+        } else {
+            __syncthreads();
         }
-        meet(more && edge_of(step + 1));
-        buf ^= 1;
+    }
+    float unit = I8 ? U : 1.0f;  // of the sums
+    if constexpr (WT > 1) {
+        // the shares' sums, in units of 2^(their largest m); the buffers are
+        // free since the last barrier
+        constexpr int LD = 32 * NS + 4;
+        float *const s_ml = reinterpret_cast<float *>(s_kv);  // [WT][M][2]
+        float *const s_o = s_ml + WT * M * 2;                 // [WT / 2][M][LD]
+        static_assert((WT * M * 2 + WT / 2 * M * LD) * 4 <= sizeof(s_kv), "the buffers hold the sums");
+        const int mine = 32 * wr + row;
+        l = pair_sum(l);
+        if (g == 0) {
+            s_ml[(wt * M + mine) * 2] = m;
+            s_ml[(wt * M + mine) * 2 + 1] = l;
+        }
+        __syncthreads();
+        float top = kNone;
+#pragma unroll
+        for (int w = 0; w < WT; w++) top = fmaxf(top, s_ml[(w * M + mine) * 2]);
+        const float f = __builtin_amdgcn_exp2f(m - top) * unit;
+        l = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WT; w++)
+            l = __builtin_fmaf(s_ml[(w * M + mine) * 2 + 1],
+                               __builtin_amdgcn_exp2f(s_ml[(w * M + mine) * 2] - top), l);
+        l *= 0.5f;  // pair_sum adds it up again
+        m = top;
+        unit = 1.0f;
+#pragma unroll
+        for (int d = 0; d < NS; d++) acc[d] *= f;
+#pragma unroll
+        for (int from = WT / 2; from >= 1; from /= 2) {
+            if (wt >= from && wt < 2 * from) {
+                float *o = s_o + ((wt - from) * M + mine) * LD + 4 * g;
+#pragma unroll
+                for (int d = 0; d < NS; d++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        *reinterpret_cast<floatx4 *>(o + 32 * d + 8 * e) =
+                            floatx4{acc[d][4 * e], acc[d][4 * e + 1], acc[d][4 * e + 2], acc[d][4 * e + 3]};
+            }
+            __syncthreads();
+            if (wt < from) {
+                const float *o = s_o + (wt * M + mine) * LD + 4 * g;
+#pragma unroll
+                for (int d = 0; d < NS; d++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const floatx4 v = *reinterpret_cast<const floatx4 *>(o + 32 * d + 8 * e);
+#pragma unroll
+                        for (int k = 0; k < 4; k++) acc[d][4 * e + k] += v[k];
+                    }
+            }
+            __syncthreads();
+        }
+        if (wt) return;
     }
     if (!valid) return;
     l = pair_sum(l);
     const int64_t orow = x.s.row0 + i;
     const int head = h * G + r % G;
-    const float unit = I8 ? U : 1.0f;
     const float inv = x.parts > 1 ? unit : l == 0.0f ? 0.0f : unit / l;
     const int64_t at = (orow * a.H + head) * t.splits + split;
+    const auto out = [&](auto put) {
 #pragma unroll
-    for (int d = 0; d < NS; d++)
+        for (int d = 0; d < NS; d++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const int dim = 32 * d + 8 * e + 4 * g;
-            const floatx4 o = floatx4{acc[d][4 * e], acc[d][4 * e + 1], acc[d][4 * e + 2],
-                                      acc[d][4 * e + 3]} * inv;
-            if (x.parts > 1)
-                *reinterpret_cast<floatx4 *>(t.part_o + at * (32 * NS) + dim) = o;
-            else if (dim < a.hd)
-                store4_any(ACT, t.out, orow * t.ldo + (int64_t)head * a.hd + dim, t.vec, o);
-        }
+            for (int e = 0; e < 4; e++)
+                put(32 * d + 8 * e + 4 * g, floatx4{acc[d][4 * e], acc[d][4 * e + 1], acc[d][4 * e + 2],
+                                                    acc[d][4 * e + 3]} * inv);
+    };
+    const int64_t to = orow * t.ldo + (int64_t)head * a.hd;
+    if (x.parts > 1)
+        out([&](int dim, floatx4 o) { *reinterpret_cast<floatx4 *>(t.part_o + at * (32 * NS) + dim) = o; });
+    else if (t.vec)
+        out([&](int dim, floatx4 o) { if (dim < a.hd) store4_any(ACT, t.out, to + dim, true, o); });
+    else
+        out([&](int dim, floatx4 o) { if (dim < a.hd) store4_any(ACT, t.out, to + dim, false, o); });
     if (x.parts > 1 && g == 0) {
         t.part_ml[2 * at] = m;
         t.part_ml[2 * at + 1] = l;
@@ -498,21 +585,18 @@ __global__ __launch_bounds__(64 * W, W == 8 ? 2 : 1) void k_attend_prompt(KvArgs
 }
 
 template <int ACT>
-hipError_t prompt_launch(const KvArgs &a, const AttendArgs &t, int tiles, int waves, hipStream_t st) {
+hipError_t prompt_launch(const KvArgs &a, const AttendArgs &t, int tiles, bool many, hipStream_t st) {
     const dim3 grid((unsigned)tiles * a.KVH, t.splits);
-    const auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(64 * waves), 0, st, a, t); };
+    const auto go = [&](auto kern, int waves) { hipLaunchKernelGGL(kern, grid, dim3(64 * waves), 0, st, a, t); };
     by_dims(a, [&](auto ns) {
-        constexpr int NS = decltype(ns)::value;
-        if constexpr (NS <= 4) {  // 2 waves or 8
-            if (waves == 2) a.i8 ? go(k_attend_prompt<ACT, true, NS, 2>) : go(k_attend_prompt<ACT, false, NS, 2>);
-            else a.i8 ? go(k_attend_prompt<ACT, true, NS, 8>) : go(k_attend_prompt<ACT, false, NS, 8>);
-        } else {  // 4: two would hold too much of a step in registers, eight too much of q
-            a.i8 ? go(k_attend_prompt<ACT, true, NS, 4>) : go(k_attend_prompt<ACT, false, NS, 4>);
-        }
+        constexpr int NS = decltype(ns)::value, MANY = kManyRows<NS>, SHARES = kShares<NS>;
+        if (many) a.i8 ? go(k_attend_prompt<ACT, true, NS, MANY, 1>, MANY) : go(k_attend_prompt<ACT, false, NS, MANY, 1>, MANY);
+        else a.i8 ? go(k_attend_prompt<ACT, true, NS, 2, SHARES>, 2 * SHARES) : go(k_attend_prompt<ACT, false, NS, 2, SHARES>, 2 * SHARES);
     });
-    return waves == 2   ? attend_join<64, 64, kPromptLeast>(a, t, tiles, st)
-           : waves == 4 ? attend_join<64, 128, kPromptLeast>(a, t, tiles, st)
-                        : attend_join<64, 256, kPromptLeast>(a, t, tiles, st);
+    if (many) return a.hdp <= 128 ? attend_join<64, 256, kPromptLeast<1>>(a, t, tiles, st)
+                                  : attend_join<64, 128, kPromptLeast<1>>(a, t, tiles, st);
+    return a.hdp <= 128 ? attend_join<64, 64, kPromptLeast<kShares<4>>>(a, t, tiles, st)
+                        : attend_join<64, 64, kPromptLeast<kShares<8>>>(a, t, tiles, st);
 }
 
 }  // namespace lcmoe

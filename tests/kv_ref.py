@@ -248,8 +248,9 @@ class Rig:
         assert (flat[:offset] == 7).all() and (got[:, row:] == 7).all() and (got[N:] == 7).all()
         return from_bits(got[:N, :row], self.act).reshape(N, self.H, self.hd)
 
-    def check_attention(self, lens, new, pages, q, scale=None, got=None, **kw):
-        """Against float64, to a bound that counts the kernel's roundings."""
+    def check_attention(self, lens, new, pages, q, scale=None, got=None, every=1, **kw):
+        """Against float64, to a bound that counts the kernel's roundings; of
+        each sequence's rows the last and `every` so many."""
         got = self.attention(lens, new, pages, q, scale, **kw) if got is None else got
         scale = self.hd ** -0.5 if scale is None else scale
         qs = self._rotated(from_bits(to_bits(q, self.act), self.act), lens, new)
@@ -261,6 +262,9 @@ class Rig:
             k, there = self.ref.values(0, pages[b], n)
             v, _ = self.ref.values(1, pages[b], n)
             for i in range(new[b]):
+                if (new[b] - 1 - i) % every:
+                    at += 1
+                    continue
                 want, size, *by = attend(qs[at], k, v, lens[b] + i, there, scale)
                 vmax = np.abs(v[there]).max(initial=0.0)
                 tol = self.bound(size, *by, vmax) + HALF_STEP[self.act] * (np.abs(want) + size * 2.0**-9)

@@ -142,6 +142,54 @@ def test_prompt(kv):
     rig.check_attention([0, 0], new, pages, normal(rng, 1159, 8, 128))
 
 
+# enough rows that a block takes many of them at a time
+@pytest.mark.parametrize("kv", ["i8", "f16"])
+@pytest.mark.parametrize("act,hd,lens,new", [
+    ("f32", 64, [0, 300], [700, 331]), ("bf16", 128, [70, 0, 5], [601, 1, 300]),
+    ("f16", 96, [129], [1000]), ("bf16", 48, [0], [1025]), ("f32", 256, [0, 33], [500, 200]),
+    ("f16", 160, [64], [600])])
+def test_many_rows(kv, act, hd, lens, new):
+    rng = np.random.default_rng(hd)
+    held = [-(-(a + b) // 32) for a, b in zip(lens, new)]
+    rig = Rig(24, 24, hd, 32, kv, act, sum(held), max(held))
+    pages = tables(rng, rig.n_pages, rig.max_pages, held)
+    if any(lens):
+        fill(rig, rng, lens, pages)
+    N = sum(new)
+    rig.append(lens, new, pages, normal(rng, N, 24, hd), normal(rng, N, 24, hd))
+    rig.check_attention(lens, new, pages, normal(rng, N, 24, hd, scale=2.0), every=7)
+
+
+@pytest.mark.parametrize("kv", ["i8", "f16"])
+def test_many_rows_and_a_missing_page(kv):
+    rng = np.random.default_rng(20)
+    rig = Rig(24, 24, 64, 16, kv, "f32", 80, 70)
+    pages = tables(rng, 80, 70, [70])
+    pages[0, [3, 40]] = -1, 80
+    x = normal(rng, 1100, 24, 64), normal(rng, 1100, 24, 64)
+    rig.append([0], [1100], pages, *x)
+    rig.check_attention([0], [1100], pages, normal(rng, 1100, 24, 64), every=5)
+
+
+@pytest.mark.parametrize("bad", [np.inf, np.nan])
+def test_many_rows_and_nonfinite_values(bad):
+    rng = np.random.default_rng(21)
+    rig = Rig(24, 24, 64, 16, "f16", "f32", 80, 70)
+    pages = tables(rng, 80, 70, [70])
+    k, v, q = (normal(rng, 1100, 24, 64) for _ in range(3))
+    rig.append([0], [1100], pages, k, v)
+    clean = rig.attention([0], [1100], pages, q)
+    for tok, head, d in ((37, 3, 5), (511, 3, 63), (512, 7, 0), (1090, 23, 33)):
+        v[tok, head, d] = bad
+    rig.append([0], [1100], pages, k, v)
+    got = rig.attention([0], [1100], pages, q)
+    want = clean.copy()
+    for tok, head, d in ((37, 3, 5), (511, 3, 63), (512, 7, 0), (1090, 23, 33)):
+        assert not np.isfinite(got[tok:, head, d]).any()
+        got[tok:, head, d] = want[tok:, head, d]
+    np.testing.assert_array_equal(got, want)
+
+
 @pytest.mark.parametrize("kv", ["i8", "f16"])
 @pytest.mark.parametrize("new", [1, 30])
 def test_missing_pages(kv, new):
