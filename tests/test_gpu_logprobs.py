@@ -121,6 +121,27 @@ def test_the_largest_in_a_thread(V):
     check(x, np.zeros((5, 1), int), 32, "f32")
 
 
+@pytest.mark.parametrize("act,V", [("f32", 8192), ("f32", 32768), ("f32", 100003), ("f16", 32768)])
+def test_large_ones_side_by_side(act, V):
+    """4 of every 64 groups of 16 bytes hold all of the largest, so that a
+    bound from the largest element of each group's lane lies below them all."""
+    rng = np.random.default_rng(V)
+    g = 4 if act == "f32" else 8
+    x = rng.random((3, V))
+    x[(slice(None), np.arange(V) // g % 64 < 4)] += 5
+    check(to_bits(x.astype(np.float32), act), np.zeros((3, 1), int), 32, act)
+
+
+@pytest.mark.parametrize("span", [8192, 32768])
+def test_large_ones_in_every_part(span):
+    """31 of the largest in each of 40 parts of a row, and 40 in one."""
+    rng = np.random.default_rng(span)
+    x = rng.random((40, span)).astype(np.float32)
+    for r in range(40):
+        x[r, rng.choice(span, 40 if r == 17 else 31, replace=False)] += 5
+    check(x.reshape(1, -1), np.zeros((1, 1), int), 32, "f32")
+
+
 @pytest.mark.parametrize("V", [100, 5000, 200000])
 def test_masked_and_nonfinite(V):
     rng = np.random.default_rng(V)
