@@ -59,11 +59,11 @@ int64_t kv_attention_floats(const KvArgs &a) {
 }
 
 hipError_t launch_kv_attention(const KvArgs &a, const void *q, int64_t ldq, const float *rope,
-                               float scale, void *out, int64_t ldo, bool vec, float *ws,
+                               float scale, void *out, int64_t ldo, float *ws,
                                hipStream_t st) {
     Plan p[2];
     for (int i = 0, n = plans(a, p); i < n; i++) {
-        AttendArgs t{q, ldq, rope, scale, out, ldo, vec, p[i].splits, p[i].per_seq, p[i].lo,
+        AttendArgs t{q, ldq, rope, scale, out, ldo, p[i].splits, p[i].per_seq, p[i].lo,
                      p[i].hi, ws, ws + (int64_t)a.n_rows * a.H * p[i].splits * a.hdp};
         if ((int64_t)p[i].tiles * a.KVH > INT32_MAX) return hipErrorInvalidConfiguration;
         const bool many = p[i].rows > 64;

@@ -258,14 +258,12 @@ struct KvArgs {
     int n_pages, max_pages, rope_abs, act;
     bool i8;
 };
-// vec: rows start on 16 bytes and are whole 16-byte groups apart
 hipError_t launch_kv_append(const KvArgs &a, const void *k, int64_t ldk, const void *v, int64_t ldv,
-                            const float *rope, bool vec, hipStream_t st);
-hipError_t launch_kv_read(const KvArgs &a, void *k, int64_t ldk, void *v, int64_t ldv, bool vec,
-                          hipStream_t st);
+                            const float *rope, hipStream_t st);
+hipError_t launch_kv_read(const KvArgs &a, void *k, int64_t ldk, void *v, int64_t ldv, hipStream_t st);
 int64_t kv_attention_floats(const KvArgs &a);
 hipError_t launch_kv_attention(const KvArgs &a, const void *q, int64_t ldq, const float *rope,
-                               float scale, void *out, int64_t ldo, bool vec, float *ws,
+                               float scale, void *out, int64_t ldo, float *ws,
                                hipStream_t st);
 int64_t logprobs_bytes(int type, int rows, int vocab, int top);
 hipError_t launch_logprobs(int type, const void *x, int64_t ld, int rows, int vocab,

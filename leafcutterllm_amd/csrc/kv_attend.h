@@ -35,7 +35,6 @@ struct AttendArgs {
     float scale;
     void *out;
     int64_t ldo;
-    bool vec;
     int splits;   // blocks that may share a row
     int per_seq;  // tiles per sequence, all alike; 0: as many as its rows fill
     int lo, hi;   // sequences with lo < rows <= hi only (rows: tokens * group)
@@ -99,28 +98,16 @@ __device__ __forceinline__ float row_sum(float v) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-__device__ __forceinline__ void load8_any(int act, const void *p, int64_t e, bool vec, float (&o)[8]) {
-    if (act == LCMOE_TYPE_F32) load8<LCMOE_TYPE_F32>(p, e, vec, o);
-    else if (act == LCMOE_TYPE_F16) load8<LCMOE_TYPE_F16>(p, e, vec, o);
-    else load8<LCMOE_TYPE_BF16>(p, e, vec, o);
+__device__ __forceinline__ void load8_any(int act, const void *p, int64_t e, float (&o)[8]) {
+    if (act == LCMOE_TYPE_F32) load_n<LCMOE_TYPE_F32>(p, e, o);
+    else if (act == LCMOE_TYPE_F16) load_n<LCMOE_TYPE_F16>(p, e, o);
+    else load_n<LCMOE_TYPE_BF16>(p, e, o);
 }
-// 4 consecutive values
-__device__ __forceinline__ void store4_any(int act, void *p, int64_t e, bool vec, floatx4 v) {
-    if (act == LCMOE_TYPE_F32) {
-        float *o = static_cast<float *>(p) + e;
-        if (vec) *reinterpret_cast<floatx4 *>(o) = v;
-        else
-            for (int i = 0; i < 4; i++) o[i] = v[i];
-    } else {
-        uint32_t w[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-            w[i] = act == LCMOE_TYPE_F16 ? to16<LCMOE_TYPE_F16>(v[i]) : to_bf16(v[i]);
-        uint16_t *o = static_cast<uint16_t *>(p) + e;
-        if (vec) *reinterpret_cast<uintx2 *>(o) = uintx2{w[0] | (w[1] << 16), w[2] | (w[3] << 16)};
-        else
-            for (int i = 0; i < 4; i++) o[i] = (uint16_t)w[i];
-    }
+__device__ __forceinline__ void store4_any(int act, void *p, int64_t e, floatx4 v) {
+    const float o[4] = {v[0], v[1], v[2], v[3]};
+    if (act == LCMOE_TYPE_F32) store_n<LCMOE_TYPE_F32>(p, e, o);
+    else if (act == LCMOE_TYPE_F16) store_n<LCMOE_TYPE_F16>(p, e, o);
+    else store_n<LCMOE_TYPE_BF16>(p, e, o);
 }
 
 // byte `B` of four words, as one word
@@ -349,7 +336,7 @@ __global__ __launch_bounds__(256) void k_attend(KvArgs a, AttendArgs t) {
     for (int u = 0; u < UN; u++) load(kf[u], a.k, 0, u);
 
     stage_q<NS, M, 256>(a, t, x, h,
-        [&](int64_t e, float (&y)[8]) { load8_any(a.act, t.q, e, t.vec, y); },
+        [&](int64_t e, float (&y)[8]) { load8_any(a.act, t.q, e, y); },
         [&](int row, int c, const float (&y)[8], float most) { O::put(s_mem, row, c, y, most); },
         [&](int row, float most, float bad) { s_mul[row] = O::factor(most, t.scale) + bad; });
     __syncthreads();
@@ -598,7 +585,7 @@ __global__ __launch_bounds__(256) void k_attend(KvArgs a, AttendArgs t) {
         const int64_t row = x.s.row0 + r / G;
         const int head = h * G + r % G;
         if (x.parts == 1) {
-            store4_any(a.act, t.out, row * t.ldo + (int64_t)head * a.hd + d, t.vec,
+            store4_any(a.act, t.out, row * t.ldo + (int64_t)head * a.hd + d,
                        o * (sum == 0.0f ? 0.0f : 1.0f / sum));
         } else {
             const int64_t at = (row * a.H + head) * t.splits + split;
@@ -654,7 +641,7 @@ __global__ __launch_bounds__(256) void k_attend_join(KvArgs a, AttendArgs t) {
     for (int k = 1; k < groups; k++) o += s_o[k * C + tid];
     float l = 0.0f;
     for (int s = 0; s < x.parts; s++) l += s_l[s];
-    store4_any(a.act, t.out, row * t.ldo + (int64_t)head * a.hd + d, t.vec,
+    store4_any(a.act, t.out, row * t.ldo + (int64_t)head * a.hd + d,
                o * (l == 0.0f ? 0.0f : 1.0f / l));
 }
 

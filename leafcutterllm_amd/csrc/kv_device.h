@@ -93,37 +93,17 @@ __device__ __forceinline__ int find_tile(const KvArgs &a, int tile, Count count,
     return -1;
 }
 
-// 8 consecutive activations from element e of `base` (f32, f16 or bf16); vec:
-// every such group is 16-byte aligned
-template <int ACT>
-__device__ __forceinline__ void load8(const void *base, int64_t e, bool vec, float (&o)[8]) {
+// N (4 or 8) consecutive activations (f32, f16 or bf16) from element e of
+// `base`, which need be aligned to an element only
+template <int ACT, int N>
+__device__ __forceinline__ void load_n(const void *base, int64_t e, float (&o)[N]) {
     if constexpr (ACT == LCMOE_TYPE_F32) {
-        const float *p = static_cast<const float *>(base) + e;
-        if (vec) {
-            const floatx4 x = reinterpret_cast<const floatx4 *>(p)[0];
-            const floatx4 y = reinterpret_cast<const floatx4 *>(p)[1];
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                o[i] = x[i];
-                o[4 + i] = y[i];
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; i++) o[i] = p[i];
-        }
+        __builtin_memcpy(o, static_cast<const float *>(base) + e, 4 * N);
     } else {
-        const uint16_t *p = static_cast<const uint16_t *>(base) + e;
-        uint32_t w[4];
-        if (vec) {
-            const uintx4 x = *reinterpret_cast<const uintx4 *>(p);
+        uint32_t w[N / 2];
+        __builtin_memcpy(w, static_cast<const uint16_t *>(base) + e, 2 * N);
 #pragma unroll
-            for (int i = 0; i < 4; i++) w[i] = x[i];
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; i++) w[i] = p[2 * i] | ((uint32_t)p[2 * i + 1] << 16);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
+        for (int i = 0; i < N / 2; i++) {
             if constexpr (ACT == LCMOE_TYPE_F16) {
                 o[2 * i] = dh2f(w[i] & 0xffff);
                 o[2 * i + 1] = dh2f(w[i] >> 16);
@@ -152,25 +132,15 @@ __device__ __forceinline__ uint32_t to16(float f) {
         return to_bf16(f);
     }
 }
-template <int ACT>
-__device__ __forceinline__ void store1(void *base, int64_t e, float f) {
-    if constexpr (ACT == LCMOE_TYPE_F32) static_cast<float *>(base)[e] = f;
-    else static_cast<uint16_t *>(base)[e] = (uint16_t)to16<ACT>(f);
-}
-template <int ACT>
-__device__ __forceinline__ void store8(void *base, int64_t e, bool vec, const float (&o)[8]) {
-    if (!vec) {
-#pragma unroll
-        for (int i = 0; i < 8; i++) store1<ACT>(base, e + i, o[i]);
-    } else if constexpr (ACT == LCMOE_TYPE_F32) {
-        floatx4 *p = reinterpret_cast<floatx4 *>(static_cast<float *>(base) + e);
-        p[0] = floatx4{o[0], o[1], o[2], o[3]};
-        p[1] = floatx4{o[4], o[5], o[6], o[7]};
+template <int ACT, int N>
+__device__ __forceinline__ void store_n(void *base, int64_t e, const float (&o)[N]) {
+    if constexpr (ACT == LCMOE_TYPE_F32) {
+        __builtin_memcpy(static_cast<float *>(base) + e, o, 4 * N);
     } else {
-        uintx4 w;
+        uint32_t w[N / 2];
 #pragma unroll
-        for (int i = 0; i < 4; i++) w[i] = to16<ACT>(o[2 * i]) | (to16<ACT>(o[2 * i + 1]) << 16);
-        *reinterpret_cast<uintx4 *>(static_cast<uint16_t *>(base) + e) = w;
+        for (int i = 0; i < N / 2; i++) w[i] = to16<ACT>(o[2 * i]) | (to16<ACT>(o[2 * i + 1]) << 16);
+        __builtin_memcpy(static_cast<uint16_t *>(base) + e, w, 2 * N);
     }
 }
 

@@ -273,7 +273,7 @@ __global__ __launch_bounds__(64 * WR * WT, NS <= 4 ? 2 : 1) void k_attend_prompt
     // its operands, through LDS: [group of rows][piece][16 dims][lane]
     half8 *const s_q = s_kv;
     stage_q<NS, M, 64 * WR * WT>(a, t, x, h,
-        [&](int64_t e, float (&y)[8]) { load8<ACT>(t.q, e, t.vec, y); },
+        [&](int64_t e, float (&y)[8]) { load_n<ACT>(t.q, e, y); },
         [&](int r, int c, const float (&y)[8], float most) {
             half8 o[NQ];
             half_pieces<NQ>(y, exponent_of(most), o);
@@ -574,10 +574,8 @@ __global__ __launch_bounds__(64 * WR * WT, NS <= 4 ? 2 : 1) void k_attend_prompt
     const int64_t to = orow * t.ldo + (int64_t)head * a.hd;
     if (x.parts > 1)
         out([&](int dim, floatx4 o) { *reinterpret_cast<floatx4 *>(t.part_o + at * (32 * NS) + dim) = o; });
-    else if (t.vec)
-        out([&](int dim, floatx4 o) { if (dim < a.hd) store4_any(ACT, t.out, to + dim, true, o); });
     else
-        out([&](int dim, floatx4 o) { if (dim < a.hd) store4_any(ACT, t.out, to + dim, false, o); });
+        out([&](int dim, floatx4 o) { if (dim < a.hd) store4_any(ACT, t.out, to + dim, o); });
     if (x.parts > 1 && g == 0) {
         t.part_ml[2 * at] = m;
         t.part_ml[2 * at + 1] = l;

@@ -118,9 +118,6 @@ lcmoe_status check_rows(const char *name, const void *p, int64_t ld, int heads,
                     (long long)ld, heads, d->head_dim);
     return LCMOE_OK;
 }
-bool wide(const void *p, int64_t ld, int act) {
-    return !((uintptr_t)p & 15) && ld * act_bytes(act) % 16 == 0;
-}
 
 KvArgs args_of(const lcmoe_kv_desc *d, const lcmoe_kv_pool *p, const lcmoe_kv_batch *b) {
     KvArgs a{};
@@ -193,8 +190,7 @@ extern "C" lcmoe_status lcmoe_kv_append_dev(const lcmoe_kv_desc *desc, const lcm
     if (lcmoe_status s = check_rope(rope_dev)) return s;
     OnDeviceOf on(stream);
     HIP_TRY(on.err);
-    const bool vec = wide(k_dev, ld_k, desc->act_type) && wide(v_dev, ld_v, desc->act_type);
-    HIP_TRY(launch_kv_append(args_of(desc, pool, batch), k_dev, ld_k, v_dev, ld_v, rope_dev, vec,
+    HIP_TRY(launch_kv_append(args_of(desc, pool, batch), k_dev, ld_k, v_dev, ld_v, rope_dev,
                              (hipStream_t)stream));
     return LCMOE_OK;
 }
@@ -211,8 +207,7 @@ extern "C" lcmoe_status lcmoe_kv_read_dev(const lcmoe_kv_desc *desc, const lcmoe
     if (lcmoe_status s = check_rows("v", v_dev, ld_v, desc->n_kv_head, desc)) return s;
     OnDeviceOf on(stream);
     HIP_TRY(on.err);
-    const bool vec = wide(k_dev, ld_k, desc->act_type) && wide(v_dev, ld_v, desc->act_type);
-    HIP_TRY(launch_kv_read(args_of(desc, pool, batch), k_dev, ld_k, v_dev, ld_v, vec,
+    HIP_TRY(launch_kv_read(args_of(desc, pool, batch), k_dev, ld_k, v_dev, ld_v,
                            (hipStream_t)stream));
     return LCMOE_OK;
 }
@@ -251,8 +246,7 @@ extern "C" lcmoe_status lcmoe_kv_attention_dev(const lcmoe_kv_desc *desc, const 
                     need, workspace ? workspace_bytes : 0);
     OnDeviceOf on(stream);
     HIP_TRY(on.err);
-    const bool vec = wide(q_dev, ld_q, desc->act_type) && wide(out_dev, ld_out, desc->act_type);
-    HIP_TRY(launch_kv_attention(a, q_dev, ld_q, rope_dev, scale, out_dev, ld_out, vec,
+    HIP_TRY(launch_kv_attention(a, q_dev, ld_q, rope_dev, scale, out_dev, ld_out,
                                 static_cast<float *>(workspace), (hipStream_t)stream));
     return LCMOE_OK;
 }
