@@ -373,6 +373,17 @@ typedef struct lcmoe_model lcmoe_model;
  * Q4_K cannot hold as zero is stored as its sanitised f32 dequantisation. */
 lcmoe_status lcmoe_model_create(const lcmoe_model_desc *desc, const lcmoe_model_weights *w,
                                 lcmoe_model **out);
+/* The same model with its cache in pages of page_tokens tokens (16, 32, 64, 128
+ * or 256) that the sequences share: kv_type LCMOE_TYPE_F16 or LCMOE_TYPE_I8 (8
+ * bits, see lcmoe_kv_desc), n_pages pages per layer, 0: enough for max_batch
+ * sequences of max_ctx.  Sequences take pages as they grow and give them back
+ * at a reset (lcmoe_model_generate's included); a call for which too few are
+ * free returns LCMOE_ERR_OUT_OF_MEMORY before it changes anything but, in
+ * lcmoe_model_generate, the caches that it clears.  Keys, values and attention
+ * run through lcmoe_kv_append_dev and lcmoe_kv_attention_dev. */
+lcmoe_status lcmoe_model_create_paged(const lcmoe_model_desc *desc, const lcmoe_model_weights *w,
+                                      int32_t kv_type, int32_t page_tokens, int32_t n_pages,
+                                      lcmoe_model **out);
 void lcmoe_model_destroy(lcmoe_model *m);
 /* KVCache::clear (cache/mod.rs:27-31) for every sequence. */
 lcmoe_status lcmoe_model_reset(lcmoe_model *m);
@@ -384,8 +395,20 @@ lcmoe_status lcmoe_model_reset(lcmoe_model *m);
  * (engine.rs:138). */
 lcmoe_status lcmoe_model_forward(lcmoe_model *m, const int32_t *tokens, int32_t B, int32_t T,
                                  float *logits);
-/* A forward or generate that fails after enqueueing device work leaves the
- * model refusing lcmoe_model_forward with LCMOE_ERR_STATE until
+/* lcmoe_model_forward with, instead of the last token's logits, what
+ * lcmoe_logprobs_dev says of every token's: logprobs [B, T] the log probability
+ * of targets [B, T] after each token (0 for a target outside [0, vocab); the
+ * text's own next tokens give its log likelihood), entropy [B, T] (NULL: not
+ * wanted), the n_top likeliest ids and their log probabilities [B, T, n_top].
+ * targets and logprobs may both be NULL.  The tokens enter the caches, so a
+ * long text is scored in calls of up to max_prompt.  The first call allocates
+ * its buffers (256 rows of logits).  No counterpart in the reference, whose
+ * forward keeps the last token's logits alone (engine.rs:117-131). */
+lcmoe_status lcmoe_model_score(lcmoe_model *m, const int32_t *tokens, const int32_t *targets,
+                               int32_t B, int32_t T, float *logprobs, float *entropy,
+                               int32_t n_top, int32_t *top_ids, float *top_logprobs);
+/* A forward, score or generate that fails after enqueueing device work leaves the
+ * model refusing lcmoe_model_forward and _score with LCMOE_ERR_STATE until
  * lcmoe_model_reset (the cache lengths on the device may have advanced);
  * lcmoe_model_generate resets by itself. */
 /* Engine::generate (engine.rs:51-76) with greedy sampling for B sequences

@@ -37,7 +37,7 @@ EXPORTS = (
     "lcmoe_gguf_moe_layer", "lcmoe_set_norm", "lcmoe_forward_norm_residual",
     "lcmoe_forward_norm_residual_dev", "lcmoe_debug_rmsnorm", "lcmoe_shard_matmul",
     "lcmoe_shard_matmul_dev", "lcmoe_shard_matmul_split_dev",
-    "lcmoe_shard_matmul_split_noalloc_dev", "lcmoe_model_create", "lcmoe_model_destroy",
+    "lcmoe_shard_matmul_split_noalloc_dev", "lcmoe_model_create", "lcmoe_model_create_paged", "lcmoe_model_score", "lcmoe_model_destroy",
     "lcmoe_model_reset", "lcmoe_model_forward", "lcmoe_model_generate",
     "lcmoe_model_last_timing", "lcmoe_model_set_decode_graph", "lcmoe_matmul_f32",
     "lcmoe_matmul_f32_dev", "lcmoe_debug_route_fallbacks", "lcmoe_debug_read_bandwidth",

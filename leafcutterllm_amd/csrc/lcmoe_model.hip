@@ -3,7 +3,8 @@
 // (rust/src/inference/engine.rs:51-132) on one GPU, with every layer's FFN
 // through the MoE layer (lcmoe_forward_norm_residual_dev).  Weights are
 // resident from lcmoe_model_create; each sequence of a batch keeps its own
-// f16 KV cache.  A decode step reads the cache lengths and the previous
+// f16 KV cache, or takes pages of a shared pool (lcmoe_model_create_paged).  A
+// decode step reads the cache lengths and the previous
 // tokens from device memory, so its launch sequence never changes: it is
 // captured once into a HIP graph and replayed for every step.
 
@@ -40,6 +41,7 @@ struct lcmoe_model {
         uint8_t *wqkv_r = nullptr, *wo_r = nullptr;
         float *attn_norm = nullptr;
         lcmoe_handle *moe = nullptr;
+        lcmoe_kv_pool pool{};  // of a paged model
     };
     std::vector<Layer> layers;
     uint8_t *embd = nullptr, *out_w = nullptr, *out_r = nullptr;
@@ -48,6 +50,17 @@ struct lcmoe_model {
     float *lpart = nullptr;                    // their K-slice partials
     float *out_norm = nullptr, *freq = nullptr;
     _Float16 *kc = nullptr, *vc = nullptr;  // [layer][seq][ctx][kv head][head_dim]
+    // A paged model has pools instead, one page table for all layers: page
+    // ids are taken from free_pages as a sequence grows, on the host and
+    // before a call's work is enqueued, and go back at a reset.
+    bool paged = false;
+    lcmoe_kv_desc kv{};
+    int32_t *pages = nullptr;             // [max_batch][kv.max_pages]
+    std::vector<int32_t> pages_h, held;   // mirror; pages of each sequence
+    std::vector<int32_t> free_pages;
+    float *rope = nullptr;
+    void *kv_ws = nullptr;
+    size_t kv_ws_bytes = 0;
     int32_t *lens = nullptr, *step = nullptr, *tok = nullptr, *next = nullptr, *out_tok = nullptr;
     float *hidden = nullptr, *xn = nullptr, *qkv = nullptr, *qr = nullptr, *attn = nullptr,
           *part = nullptr, *logits = nullptr;
@@ -62,6 +75,15 @@ struct lcmoe_model {
     bool use_graph = true;
     hipEvent_t ev[4] = {nullptr, nullptr, nullptr, nullptr};  // start, prefilled, decode, end
     double prefill_ms = 0, decode_ms = 0;
+    // lcmoe_model_score, allocated by its first call: `rows` rows at a time
+    struct Score {
+        int rows = 0;
+        float *logits = nullptr, *part = nullptr, *lp = nullptr, *entropy = nullptr,
+              *top_lp = nullptr;
+        int32_t *targets = nullptr, *top_id = nullptr;
+        void *ws = nullptr;
+        size_t ws_bytes = 0;
+    } score;
 };
 
 namespace {
@@ -179,13 +201,33 @@ lcmoe_status validate(const lcmoe_model_desc *d, const lcmoe_model_weights *w) {
     return LCMOE_OK;
 }
 
-// Rows [q0, q0 + nq) of the batch forward.  nseq sequences starting at seq0
-// take T tokens each from tok (nseq == 1 or T == 1); their last tokens'
-// logits land in m->logits rows 0 .. nseq-1, the greedy ids in m->next
-// (and, with rec, in m->out_tok at column *m->step); the cache lengths
-// advance by T and *m->step by dstep.
-lcmoe_status forward_dev(lcmoe_model *m, int seq0, int nseq, int T, const int32_t *tok, bool rec,
-                         int dstep) {
+// Y (= or R +) X W^T over `rows` rows of X (ld K): the matrix-core linear for
+// batches of rows when W has its RPL64 copy, else launch_linear
+hipError_t linear(lcmoe_model *m, int wt, const uint8_t *W, const uint8_t *Wr, int N, int K,
+                  const float *X, int rows, const float *R, float *Y, int64_t ldy, float *part) {
+    if (Wr && rows >= 2)
+        return launch_linear_mfma(Wr, N, K, X, rows, R, Y, ldy, m->x16, m->xs16, part, m->stream);
+    return launch_linear(wt, W, N, K, X, K, rows, R, Y, ldy, m->stream);
+}
+
+// A layer's attention over its pool: the keys and values of m->qkv appended,
+// m->attn of its queries.
+lcmoe_status attend_paged(lcmoe_model *m, const lcmoe_kv_pool &pool, int seq0, int nseq, int T) {
+    const lcmoe_kv_desc &K = m->kv;
+    const int64_t ld = (int64_t)(K.n_head + 2 * K.n_kv_head) * K.head_dim;
+    const lcmoe_kv_batch b{nseq, nseq * T, T, nullptr, m->lens + seq0,
+                           m->pages + (int64_t)seq0 * K.max_pages};
+    const float *k = m->qkv + (int64_t)K.n_head * K.head_dim, *v = k + (int64_t)K.n_kv_head * K.head_dim;
+    lcmoe_status s = lcmoe_kv_append_dev(&K, &pool, &b, k, ld, v, ld, m->rope, m->stream);
+    if (s) return s;
+    return lcmoe_kv_attention_dev(&K, &pool, &b, m->qkv, ld, m->rope,
+                                  1.0f / std::sqrt((float)K.head_dim), m->attn,
+                                  (int64_t)K.n_head * K.head_dim, m->kv_ws, m->kv_ws_bytes, m->stream);
+}
+
+// The layers of a forward: nseq sequences starting at seq0 take T tokens each
+// from tok (nseq == 1 or T == 1); their rows are left in m->hidden.
+lcmoe_status layers_dev(lcmoe_model *m, int seq0, int nseq, int T, const int32_t *tok) {
     if (m->fail_at >= 0 && m->fail_at-- == 0)
         return fail(LCMOE_ERR_STATE, "forward failure requested by lcmoe_model_debug_fail_forward");
     const lcmoe_model_desc &D = m->desc;
@@ -193,51 +235,64 @@ lcmoe_status forward_dev(lcmoe_model *m, int seq0, int nseq, int T, const int32_
     const int nq = nseq * T, nqkv = (H + 2 * KVH) * hd;
     const int64_t cache_layer = (int64_t)D.max_batch * D.max_ctx * KVH * hd;
     hipStream_t st = m->stream;
-    // Y (= or R +) X W^T over `rows` rows of X (ld K): the matrix-core linear
-    // for batches of rows when W has its RPL64 copy, else launch_linear
-    auto linear = [&](int wt, const uint8_t *W, const uint8_t *Wr, int N, int K, const float *X,
-                      int rows, const float *R, float *Y, int64_t ldy) {
-        if (Wr && rows >= 2)
-            return launch_linear_mfma(Wr, N, K, X, rows, R, Y, ldy, m->x16, m->xs16, m->lpart, st);
-        return launch_linear(wt, W, N, K, X, K, rows, R, Y, ldy, st);
-    };
     HIP_TRY(launch_embed(m->qt_embd, m->embd, V, d, tok, nq, m->hidden, st));
     for (int l = 0; l < D.n_layer; l++) {
         const auto &L = m->layers[l];
-        _Float16 *kc = m->kc + l * cache_layer, *vc = m->vc + l * cache_layer;
         // Batches on the matrix-core linears: the attention norm also writes
         // the QKV projection's f16 pieces, RoPE adds the projection's K
         // slices as it reads them, and the attention's combine writes the
         // output projection's pieces (no launches of their own).
         const bool mq = L.wqkv_r && nq >= 2;
-        const bool mo = L.wo_r && nq >= 2 && hd % 32 == 0 && hd <= 256;  // whole sub-blocks per head
+        const bool mo = !m->paged && L.wo_r && nq >= 2 && hd % 32 == 0 && hd <= 256;  // whole sub-blocks per head
         HIP_TRY(launch_rmsnorm(m->hidden, L.attn_norm, D.norm_eps, nq, d, m->xn, st,
                                mq ? m->x16 : nullptr, m->xs16));
         int ks = 1;
         if (mq)
             HIP_TRY(launch_linear_mfma(L.wqkv_r, nqkv, d, nullptr, nq, nullptr, m->qkv, nqkv,
-                                       m->x16, m->xs16, m->lpart, st, true, &ks));
+                                       m->x16, m->xs16, m->lpart, st, true, m->paged ? nullptr : &ks));
         else
-            HIP_TRY(linear(L.qt_qkv, L.wqkv, nullptr, nqkv, d, m->xn, nq, nullptr, m->qkv, nqkv));
-        HIP_TRY(launch_rope_kv(ks > 1 ? m->lpart : m->qkv, nq, T, seq0, m->lens, H, KVH, hd,
-                               m->freq, D.rope_positions == LCMOE_ROPE_ABSOLUTE, m->qr, kc, vc,
-                               D.max_ctx, st, ks, (int64_t)nq * nqkv));
-        HIP_TRY(launch_attention(m->qr, nq, T, seq0, m->lens, H, KVH, hd, kc, vc, D.max_ctx,
-                                 m->part, m->attn, st, mo ? m->x16 : nullptr, m->xs16));
+            HIP_TRY(linear(m, L.qt_qkv, L.wqkv, nullptr, nqkv, d, m->xn, nq, nullptr, m->qkv, nqkv,
+                           m->lpart));
+        if (m->paged) {
+            lcmoe_status s = attend_paged(m, L.pool, seq0, nseq, T);
+            if (s) return s;
+        } else {
+            _Float16 *kc = m->kc + l * cache_layer, *vc = m->vc + l * cache_layer;
+            HIP_TRY(launch_rope_kv(ks > 1 ? m->lpart : m->qkv, nq, T, seq0, m->lens, H, KVH, hd,
+                                   m->freq, D.rope_positions == LCMOE_ROPE_ABSOLUTE, m->qr, kc, vc,
+                                   D.max_ctx, st, ks, (int64_t)nq * nqkv));
+            HIP_TRY(launch_attention(m->qr, nq, T, seq0, m->lens, H, KVH, hd, kc, vc, D.max_ctx,
+                                     m->part, m->attn, st, mo ? m->x16 : nullptr, m->xs16));
+        }
         // hidden += attn W_o (Tensor::add, engine.rs:106)
         if (mo)
             HIP_TRY(launch_linear_mfma(L.wo_r, d, H * hd, nullptr, nq, m->hidden, m->hidden, d,
                                        m->x16, m->xs16, m->lpart, st, true));
         else
-            HIP_TRY(linear(L.qt_o, L.wo, L.wo_r, d, H * hd, m->attn, nq, m->hidden, m->hidden, d));
+            HIP_TRY(linear(m, L.qt_o, L.wo, L.wo_r, d, H * hd, m->attn, nq, m->hidden, m->hidden, d,
+                           m->lpart));
         // hidden += ffn(rms_norm(hidden)) (engine.rs:109-115)
         lcmoe_status s = lcmoe_forward_norm_residual_dev(L.moe, m->hidden, nq, m->hidden, st);
         if (s) return s;
     }
+    return LCMOE_OK;
+}
+
+// A forward of nseq sequences starting at seq0, T tokens each from tok (nseq
+// == 1 or T == 1); their last tokens' logits land in m->logits rows 0 ..
+// nseq-1, the greedy ids in m->next (and, with rec, in m->out_tok at column
+// *m->step); the cache lengths advance by T and *m->step by dstep.
+lcmoe_status forward_dev(lcmoe_model *m, int seq0, int nseq, int T, const int32_t *tok, bool rec,
+                         int dstep) {
+    lcmoe_status s = layers_dev(m, seq0, nseq, T, tok);
+    if (s) return s;
+    const lcmoe_model_desc &D = m->desc;
+    const int d = D.d_model, V = D.vocab;
+    hipStream_t st = m->stream;
     // the final norm and lm_head of each sequence's last token
     const float *last = m->hidden + (int64_t)(T - 1) * d;  // nseq == 1, or T == 1
     HIP_TRY(launch_rmsnorm(last, m->out_norm, D.norm_eps, nseq, d, m->xn, st));
-    HIP_TRY(linear(m->qt_out, m->out_w, m->out_r, V, d, m->xn, nseq, nullptr, m->logits, V));
+    HIP_TRY(linear(m, m->qt_out, m->out_w, m->out_r, V, d, m->xn, nseq, nullptr, m->logits, V, m->lpart));
     HIP_TRY(launch_argmax(m->logits, nseq, V, seq0, m->next, rec ? m->out_tok : nullptr,
                           D.max_ctx, m->step, st));
     HIP_TRY(launch_advance(m->lens, seq0, nseq, T, m->step, dstep, st));
@@ -254,6 +309,11 @@ lcmoe_status reset(lcmoe_model *m) {
     // drain whatever a failed call left queued before rewriting the lengths
     HIP_TRY(hipStreamSynchronize(m->stream));
     std::fill(m->lens_h.begin(), m->lens_h.end(), 0);
+    if (m->paged) {
+        m->free_pages.clear();
+        for (int i = m->kv.n_pages; i > 0; i--) m->free_pages.push_back(i - 1);
+        std::fill(m->held.begin(), m->held.end(), 0);
+    }
     HIP_TRY(hipMemcpyAsync(m->lens, m->lens_h.data(), 4 * m->lens_h.size(), hipMemcpyHostToDevice,
                            m->stream));
     lcmoe_status st = set_step(m, 0);
@@ -267,6 +327,37 @@ lcmoe_status reset(lcmoe_model *m) {
 lcmoe_status failed_after_enqueue(lcmoe_model *m, lcmoe_status st) {
     m->needs_reset = true;
     return st;
+}
+
+int32_t pages_for(const lcmoe_model *m, int64_t tokens) {
+    return (int32_t)((tokens + m->kv.page_tokens - 1) / m->kv.page_tokens);
+}
+
+// Pages of sequences 0 .. B-1 for T tokens more each; with too few, nothing is
+// taken and nothing enqueued.
+lcmoe_status pages_missing(const lcmoe_model *m, int B, int T) {
+    if (!m->paged) return LCMOE_OK;
+    int64_t need = 0;
+    for (int b = 0; b < B; b++) need += pages_for(m, (int64_t)m->lens_h[b] + T) - m->held[b];
+    if (need > (int64_t)m->free_pages.size())
+        return fail(LCMOE_ERR_OUT_OF_MEMORY, "%lld pages needed, %zu of %d free: lcmoe_model_reset, "
+                    "or a pool of more pages", (long long)need, m->free_pages.size(), m->kv.n_pages);
+    return LCMOE_OK;
+}
+lcmoe_status take_pages(lcmoe_model *m, int B, int T) {
+    if (!m->paged) return LCMOE_OK;
+    const int32_t M = m->kv.max_pages;
+    for (int b = 0; b < B; b++) {
+        const int32_t had = m->held[b], n = pages_for(m, (int64_t)m->lens_h[b] + T);
+        if (n == had) continue;
+        for (; m->held[b] < n; m->held[b]++) {
+            m->pages_h[(size_t)b * M + m->held[b]] = m->free_pages.back();
+            m->free_pages.pop_back();
+        }
+        HIP_TRY(hipMemcpyAsync(m->pages + (int64_t)b * M + had, &m->pages_h[(size_t)b * M + had],
+                               4 * (size_t)(n - had), hipMemcpyHostToDevice, m->stream));
+    }
+    return LCMOE_OK;
 }
 
 // Engine::generate's device work after the reset: prefill each sequence,
@@ -355,15 +446,132 @@ lcmoe_status forward_tokens(lcmoe_model *m, const int32_t *tokens, int B, int T,
     return LCMOE_OK;
 }
 
+// that sequences 0 .. B-1 can take T tokens more each
+lcmoe_status takes(const lcmoe_model *m, int B, int T) {
+    const lcmoe_model_desc &D = m->desc;
+    if (B < 1 || B > D.max_batch) return fail(LCMOE_ERR_INVALID_ARG, "B=%d outside [1, %d]", B, D.max_batch);
+    if (T < 1 || T > D.max_prompt) return fail(LCMOE_ERR_INVALID_ARG, "T=%d outside [1, %d]", T, D.max_prompt);
+    if (m->needs_reset)
+        return fail(LCMOE_ERR_STATE, "an earlier call failed after enqueueing work: lcmoe_model_reset first");
+    for (int b = 0; b < B; b++)
+        if (m->lens_h[b] + T > D.max_ctx)
+            return fail(LCMOE_ERR_INVALID_ARG, "sequence %d: %d cached + %d new > max_ctx=%d", b,
+                        m->lens_h[b], T, D.max_ctx);
+    return pages_missing(m, B, T);
+}
+
+// What lcmoe_model_score needs beside the model's buffers.
+lcmoe_status score_buffers(lcmoe_model *m) {
+    if (m->score.rows) return LCMOE_OK;
+    const lcmoe_model_desc &D = m->desc;
+    const int V = D.vocab, rows = std::min(m->tmax, 256);
+    auto &S = m->score;
+    S.ws_bytes = 16;
+    for (int r = 1; r <= rows; r++)
+        for (int top : {0, LCMOE_LOGPROBS_TOP}) {
+            size_t n = 0;
+            lcmoe_status st = lcmoe_logprobs_workspace(LCMOE_TYPE_F32, r, V, 1, top, &n);
+            if (st) return st;
+            S.ws_bytes = std::max(S.ws_bytes, n);
+        }
+    const size_t had = m->allocs.size(), R = rows, K = LCMOE_LOGPROBS_TOP;
+    lcmoe_status st;
+    if ((st = alloc_n(m, &S.logits, R * V)) || (st = alloc_n(m, &S.lp, R)) ||
+        (st = alloc_n(m, &S.entropy, R)) || (st = alloc_n(m, &S.targets, R)) ||
+        (st = alloc_n(m, &S.top_id, R * K)) || (st = alloc_n(m, &S.top_lp, R * K)) ||
+        (st = alloc_n(m, reinterpret_cast<uint8_t **>(&S.ws), S.ws_bytes)) ||
+        (m->out_r &&
+         (st = alloc_n(m, &S.part, linear_mfma_part_floats(V, D.d_model, rows))))) {
+        for (; m->allocs.size() > had; m->allocs.pop_back()) (void)hipFree(m->allocs.back());
+        S = {};
+        return st;
+    }
+    S.rows = rows;
+    return LCMOE_OK;
+}
+
+struct Wanted {
+    const int32_t *targets;
+    float *lp, *entropy;
+    int n_top;
+    int32_t *top_id;
+    float *top_lp;
+};
+
+// The log probabilities of m->hidden's first n rows, results from row `at` on
+// of the caller's arrays: the final norm, the lm_head product and
+// lcmoe_logprobs_dev over m->score.rows rows at a time.
+lcmoe_status score_rows(lcmoe_model *m, int n, int64_t at, const Wanted &w) {
+    const lcmoe_model_desc &D = m->desc;
+    const int d = D.d_model, V = D.vocab, K = w.n_top;
+    auto &S = m->score;
+    hipStream_t st = m->stream;
+    for (int r0 = 0; r0 < n; r0 += S.rows) {
+        const int r = std::min(S.rows, n - r0);
+        const int64_t o = at + r0;
+        HIP_TRY(launch_rmsnorm(m->hidden + (int64_t)r0 * d, m->out_norm, D.norm_eps, r, d, m->xn, st));
+        HIP_TRY(linear(m, m->qt_out, m->out_w, m->out_r, V, d, m->xn, r, nullptr, S.logits, V, S.part));
+        if (w.targets)
+            HIP_TRY(hipMemcpyAsync(S.targets, w.targets + o, 4 * (size_t)r, hipMemcpyHostToDevice, st));
+        lcmoe_status s = lcmoe_logprobs_dev(LCMOE_TYPE_F32, S.logits, V, r, V, S.targets,
+                                            w.targets ? 1 : 0, S.lp, w.entropy ? S.entropy : nullptr,
+                                            K, S.top_id, S.top_lp, S.ws, S.ws_bytes, st);
+        if (s) return s;
+        if (w.targets)
+            HIP_TRY(hipMemcpyAsync(w.lp + o, S.lp, 4 * (size_t)r, hipMemcpyDeviceToHost, st));
+        if (w.entropy)
+            HIP_TRY(hipMemcpyAsync(w.entropy + o, S.entropy, 4 * (size_t)r, hipMemcpyDeviceToHost, st));
+        if (K) {
+            HIP_TRY(hipMemcpyAsync(w.top_id + o * K, S.top_id, 4 * (size_t)r * K, hipMemcpyDeviceToHost, st));
+            HIP_TRY(hipMemcpyAsync(w.top_lp + o * K, S.top_lp, 4 * (size_t)r * K, hipMemcpyDeviceToHost, st));
+        }
+    }
+    return LCMOE_OK;
+}
+
+// lcmoe_model_score's device work, in forward_tokens' passes
+lcmoe_status score_tokens(lcmoe_model *m, const int32_t *tokens, int B, int T, const Wanted &w) {
+    const int passes = T == 1 ? 1 : B, nseq = T == 1 ? B : 1, rows = nseq * T;
+    for (int p = 0; p < passes; p++) {
+        HIP_TRY(hipMemcpyAsync(m->tok, tokens + (size_t)p * rows, 4 * (size_t)rows,
+                               hipMemcpyHostToDevice, m->stream));
+        lcmoe_status st = layers_dev(m, p, nseq, T, m->tok);
+        if (st || (st = score_rows(m, rows, (int64_t)p * rows, w))) return st;
+        HIP_TRY(launch_advance(m->lens, p, nseq, T, m->step, 0, m->stream));
+    }
+    HIP_TRY(hipStreamSynchronize(m->stream));
+    return LCMOE_OK;
+}
+
 }  // namespace
 
-extern "C" lcmoe_status lcmoe_model_create(const lcmoe_model_desc *desc,
-                                           const lcmoe_model_weights *w, lcmoe_model **out) {
+namespace {
+
+// kv: a paged model's kv_type, page_tokens and n_pages, else null
+lcmoe_status create(const lcmoe_model_desc *desc, const lcmoe_model_weights *w,
+                    const lcmoe_kv_desc *kv, lcmoe_model **out) {
     clear_error();
     if (!out) return fail(LCMOE_ERR_INVALID_ARG, "out is NULL");
     *out = nullptr;
     lcmoe_status st = validate(desc, w);
     if (st) return st;
+    lcmoe_kv_desc KV{};
+    size_t pool_bytes = 0, scale_bytes = 0;
+    if (kv) {
+        KV = *kv;
+        KV.n_head = desc->n_head;
+        KV.n_kv_head = desc->n_kv_head;
+        KV.head_dim = desc->head_dim;
+        KV.act_type = LCMOE_TYPE_F32;
+        KV.rope_positions = desc->rope_positions;
+        if (KV.page_tokens < 16) KV.max_pages = 1;  // refused below
+        else KV.max_pages = (int32_t)(((int64_t)desc->max_ctx + KV.page_tokens - 1) / KV.page_tokens);
+        if (KV.n_pages == 0) {
+            const int64_t all = (int64_t)desc->max_batch * KV.max_pages;
+            KV.n_pages = (int32_t)std::min<int64_t>(all, INT32_MAX);
+        }
+        if ((st = lcmoe_kv_sizes(&KV, &pool_bytes, &scale_bytes))) return st;
+    }
     int ndev = 0;
     if (hipGetDeviceCount(&ndev) != hipSuccess || ndev < 1) {
         (void)hipGetLastError();
@@ -447,8 +655,52 @@ extern "C" lcmoe_status lcmoe_model_create(const lcmoe_model_desc *desc,
         if ((st = lcmoe_set_act_precision(ML.moe, LCMOE_ACT_F16X2))) return bail(st);
         if ((st = lcmoe_set_norm(ML.moe, L.ffn_norm, D.norm_eps))) return bail(st);
     }
-    const int64_t cache = (int64_t)D.n_layer * D.max_batch * D.max_ctx * KVH * hd;
+    const int64_t cache = kv ? 0 : (int64_t)D.n_layer * D.max_batch * D.max_ctx * KVH * hd;
     const int64_t T = m->tmax;
+    if (kv) {
+        m->paged = true;
+        m->kv = KV;
+        const size_t table = (size_t)D.max_batch * KV.max_pages;
+        try {
+            m->pages_h.assign(table, -1);
+            m->held.assign(D.max_batch, 0);
+            m->free_pages.reserve(KV.n_pages);
+        } catch (const std::bad_alloc &) {
+            return bail(fail(LCMOE_ERR_OUT_OF_MEMORY, "host allocation failed"));
+        }
+        for (auto &L : m->layers)
+            if ((st = alloc_n(m, reinterpret_cast<uint8_t **>(&L.pool.k), pool_bytes)) ||
+                (st = alloc_n(m, reinterpret_cast<uint8_t **>(&L.pool.v), pool_bytes)) ||
+                (st = alloc_n(m, reinterpret_cast<uint8_t **>(&L.pool.scale), scale_bytes)))
+                return bail(st);
+        // apply_rotary_emb's angles as the unpaged model has them: f32
+        // products (attention.rs:13-34)
+        const int64_t n_pos = (int64_t)KV.max_pages * KV.page_tokens;
+        std::vector<float> table_h;
+        try {
+            table_h.resize((size_t)n_pos * hd);
+        } catch (const std::bad_alloc &) {
+            return bail(fail(LCMOE_ERR_OUT_OF_MEMORY, "host allocation failed"));
+        }
+        for (int64_t p = 0; p < n_pos; p++)
+            for (int i = 0; i < hd / 2; i++) {
+                const float a = (float)p * freq[i];
+                table_h[p * hd + 2 * i] = std::cos(a);
+                table_h[p * hd + 2 * i + 1] = std::sin(a);
+            }
+        if ((st = upload(m, &m->rope, table_h.data(), 4 * table_h.size()))) return bail(st);
+        // of every step and every prompt: fewer rows may be split further
+        for (int n = 1 - D.max_prompt; n <= D.max_batch; n++) {
+            const lcmoe_kv_batch b = n > 0 ? lcmoe_kv_batch{n, n, 1, nullptr, nullptr, nullptr}
+                                           : lcmoe_kv_batch{1, 1 - n, 1 - n, nullptr, nullptr, nullptr};
+            size_t bytes = 0;
+            if ((st = lcmoe_kv_attention_workspace(&KV, &b, &bytes))) return bail(st);
+            m->kv_ws_bytes = std::max(m->kv_ws_bytes, bytes);
+        }
+        if ((st = alloc_n(m, &m->pages, table)) ||
+            (st = alloc_n(m, reinterpret_cast<uint8_t **>(&m->kv_ws), m->kv_ws_bytes)))
+            return bail(st);
+    }
     if ((st = alloc_n(m, &m->kc, cache)) || (st = alloc_n(m, &m->vc, cache)) ||
         (st = alloc_n(m, &m->lens, D.max_batch)) || (st = alloc_n(m, &m->step, 1)) ||
         (st = alloc_n(m, &m->tok, T)) || (st = alloc_n(m, &m->next, D.max_batch)) ||
@@ -475,6 +727,24 @@ extern "C" lcmoe_status lcmoe_model_create(const lcmoe_model_desc *desc,
     return LCMOE_OK;
 }
 
+}  // namespace
+
+extern "C" lcmoe_status lcmoe_model_create(const lcmoe_model_desc *desc,
+                                           const lcmoe_model_weights *w, lcmoe_model **out) {
+    return create(desc, w, nullptr, out);
+}
+
+extern "C" lcmoe_status lcmoe_model_create_paged(const lcmoe_model_desc *desc,
+                                                 const lcmoe_model_weights *w, int32_t kv_type,
+                                                 int32_t page_tokens, int32_t n_pages,
+                                                 lcmoe_model **out) {
+    lcmoe_kv_desc kv{};
+    kv.kv_type = kv_type;
+    kv.page_tokens = page_tokens;
+    kv.n_pages = n_pages;
+    return create(desc, w, &kv, out);
+}
+
 extern "C" void lcmoe_model_destroy(lcmoe_model *m) { free_model(m); }
 
 extern "C" lcmoe_status lcmoe_model_reset(lcmoe_model *m) {
@@ -488,17 +758,32 @@ extern "C" lcmoe_status lcmoe_model_forward(lcmoe_model *m, const int32_t *token
                                             int32_t T, float *logits) {
     clear_error();
     if (!m || !tokens || !logits) return fail(LCMOE_ERR_INVALID_ARG, "model, tokens or logits is NULL");
-    const lcmoe_model_desc &D = m->desc;
-    if (B < 1 || B > D.max_batch) return fail(LCMOE_ERR_INVALID_ARG, "B=%d outside [1, %d]", B, D.max_batch);
-    if (T < 1 || T > D.max_prompt) return fail(LCMOE_ERR_INVALID_ARG, "T=%d outside [1, %d]", T, D.max_prompt);
-    if (m->needs_reset)
-        return fail(LCMOE_ERR_STATE, "an earlier call failed after enqueueing work: lcmoe_model_reset first");
-    for (int b = 0; b < B; b++)
-        if (m->lens_h[b] + T > D.max_ctx)
-            return fail(LCMOE_ERR_INVALID_ARG, "sequence %d: %d cached + %d new > max_ctx=%d", b,
-                        m->lens_h[b], T, D.max_ctx);
+    lcmoe_status st = takes(m, B, T);
+    if (st) return st;
     HIP_TRY(hipSetDevice(m->device));
-    lcmoe_status st = forward_tokens(m, tokens, B, T, logits);
+    if (!(st = take_pages(m, B, T))) st = forward_tokens(m, tokens, B, T, logits);
+    if (st) return failed_after_enqueue(m, st);
+    for (int b = 0; b < B; b++) m->lens_h[b] += T;
+    return LCMOE_OK;
+}
+
+extern "C" lcmoe_status lcmoe_model_score(lcmoe_model *m, const int32_t *tokens,
+                                          const int32_t *targets, int32_t B, int32_t T,
+                                          float *logprobs, float *entropy, int32_t n_top,
+                                          int32_t *top_ids, float *top_logprobs) {
+    clear_error();
+    if (!m || !tokens) return fail(LCMOE_ERR_INVALID_ARG, "model or tokens is NULL");
+    if (!targets != !logprobs) return fail(LCMOE_ERR_INVALID_ARG, "targets and logprobs go together");
+    if (n_top < 0 || n_top > LCMOE_LOGPROBS_TOP)
+        return fail(LCMOE_ERR_INVALID_ARG, "n_top=%d outside [0, %d]", n_top, LCMOE_LOGPROBS_TOP);
+    if (n_top && (!top_ids || !top_logprobs))
+        return fail(LCMOE_ERR_INVALID_ARG, "n_top=%d needs top_ids and top_logprobs", n_top);
+    lcmoe_status st = takes(m, B, T);
+    if (st) return st;
+    HIP_TRY(hipSetDevice(m->device));
+    if ((st = score_buffers(m))) return st;
+    const Wanted w{targets, logprobs, entropy, n_top, top_ids, top_logprobs};
+    if (!(st = take_pages(m, B, T))) st = score_tokens(m, tokens, B, T, w);
     if (st) return failed_after_enqueue(m, st);
     for (int b = 0; b < B; b++) m->lens_h[b] += T;
     return LCMOE_OK;
@@ -519,6 +804,8 @@ extern "C" lcmoe_status lcmoe_model_generate(lcmoe_model *m, const int32_t *prom
     // generate starts from a cleared cache, so it runs after a failed call
     lcmoe_status st;
     if ((st = reset(m))) return failed_after_enqueue(m, st);
+    if ((st = pages_missing(m, B, P + n_new - 1))) return st;
+    if ((st = take_pages(m, B, P + n_new - 1))) return failed_after_enqueue(m, st);
     if ((st = generate_dev(m, prompt, B, P, n_new, out))) return failed_after_enqueue(m, st);
     for (int b = 0; b < B; b++) {
         m->lens_h[b] = P + n_new - 1;

@@ -52,6 +52,11 @@ class ModelWeights(C.Structure):
 _SIGS = {
     "lcmoe_model_create": (C.c_int32, [C.POINTER(ModelDesc), C.POINTER(ModelWeights),
                                        C.POINTER(C.c_void_p)]),
+    "lcmoe_model_create_paged": (C.c_int32, [C.POINTER(ModelDesc), C.POINTER(ModelWeights),
+                                             C.c_int32, C.c_int32, C.c_int32,
+                                             C.POINTER(C.c_void_p)]),
+    "lcmoe_model_score": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_int32,
+                                      C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p]),
     "lcmoe_model_destroy": (None, [C.c_void_p]),
     "lcmoe_model_reset": (C.c_int32, [C.c_void_p]),
     "lcmoe_model_forward": (C.c_int32, [C.c_void_p, C.c_void_p, C.c_int32, C.c_int32,
@@ -85,9 +90,14 @@ class Model:
     d]; output absent or None ties the LM head to token_embd), output_norm (f32 [d]) and `layers`, a list of dicts with attn_norm,
     ffn_norm (f32 [d]), attn_q / attn_k / attn_v / attn_o (GGUF bytes) and
     `moe` (the arrays lcmoe_create takes: router, bias, gate, up, down and
-    the *_sh tensors)."""
+    the *_sh tensors).
 
-    def __init__(self, desc: ModelDesc, weights: dict):
+    kv_type (TYPE_F16 or TYPE_I8): the K/V cache in pages of page_tokens
+    tokens that the sequences share, n_pages of them per layer (0: enough for
+    max_batch sequences of max_ctx); None: one f16 cache per sequence."""
+
+    def __init__(self, desc: ModelDesc, weights: dict, kv_type: int | None = None,
+                 page_tokens: int = 64, n_pages: int = 0):
         L = _bound()
         self.desc = desc
         keep = []
@@ -115,7 +125,11 @@ class Model:
         w.output_norm = p(weights["output_norm"], np.float32)
         w.layers = C.cast(layers, C.c_void_p)
         h = C.c_void_p()
-        check(L.lcmoe_model_create(C.byref(desc), C.byref(w), C.byref(h)), "lcmoe_model_create")
+        if kv_type is None:
+            check(L.lcmoe_model_create(C.byref(desc), C.byref(w), C.byref(h)), "lcmoe_model_create")
+        else:
+            check(L.lcmoe_model_create_paged(C.byref(desc), C.byref(w), kv_type, page_tokens,
+                                             n_pages, C.byref(h)), "lcmoe_model_create_paged")
         self._h = h
 
     def reset(self) -> None:
@@ -129,6 +143,28 @@ class Model:
         check(_bound().lcmoe_model_forward(self._h, t.ctypes.data, B, T, out.ctypes.data),
               "lcmoe_model_forward")
         return out
+
+    def score(self, tokens, targets=None, n_top: int = 0):
+        """The tokens [B, T] enter the caches as by forward.  Returns (logprobs
+        [B, T], entropy [B, T], top_ids, top_logprobs
+        [B, T, n_top]): after
+        each token, the log probability of its target, by default the row's next
+        token (0 after the last, and for any id outside the vocabulary)."""
+        t = np.ascontiguousarray(np.atleast_2d(tokens), np.int32)
+        B, T = t.shape
+        if targets is None:
+            g = np.concatenate([t[:, 1:], np.full((B, 1), -1, np.int32)], 1)
+        else:
+            g = np.ascontiguousarray(np.atleast_2d(targets), np.int32)
+            if g.shape != t.shape:
+                raise ValueError(f"targets {g.shape} for tokens {t.shape}")
+        lp, ent = np.empty((B, T), np.float32), np.empty((B, T), np.float32)
+        ids = np.empty((B, T, max(n_top, 0)), np.int32)
+        tlp = np.empty(ids.shape, np.float32)
+        check(_bound().lcmoe_model_score(self._h, t.ctypes.data, g.ctypes.data, B, T,
+                                         lp.ctypes.data, ent.ctypes.data, n_top, ids.ctypes.data,
+                                         tlp.ctypes.data), "lcmoe_model_score")
+        return lp, ent, ids, tlp
 
     def generate(self, prompt, n_new: int, eos: int = -1):
         """Greedy Engine::generate for each row of prompt [B, P]: (ids [B,

@@ -203,3 +203,21 @@ def test_logprobs_python_refusals():
         with pytest.raises(L.LcmoeError) as e:
             L.logprobs(*args)
         assert _lib.STATUS[e.value.status] == "LCMOE_ERR_INVALID_ARG"
+
+
+def test_paged_models_refusals():
+    """What lcmoe_model_create_paged and lcmoe_model_score refuse before any
+    device work."""
+    from leafcutterllm_amd.configs import ModelConfig, small_config, synth_model
+
+    mc = ModelConfig("tiny", 1, 4, 2, 64, 32, 10000.0,
+                     small_config("m", 256, 256, 8, 2, L.ROUTE_SOFTMAX, L.TYPE_Q4_K, L.TYPE_Q4_K))
+    w = synth_model(mc, seed=1)
+    for kv in ((L.TYPE_I8, 24, 0), (L.TYPE_I8, 0, 0), (L.TYPE_I8, -16, 0), (L.TYPE_I8, 512, 0),
+               (L.TYPE_F16, 16, -1), (L.TYPE_F32, 16, 0), (L.TYPE_Q8_0, 16, 0)):
+        with pytest.raises(L.LcmoeError) as e:
+            L.Model(mc.desc(2, 16, 32), w, *kv)
+        assert _lib.STATUS[e.value.status] in ("LCMOE_ERR_INVALID_ARG", "LCMOE_ERR_UNSUPPORTED"), kv
+    t = np.zeros(4, np.int32)
+    lib = L.lib()
+    assert lib.lcmoe_model_score(None, t.ctypes.data, None, 1, 4, None, None, 0, None, None) == 1
