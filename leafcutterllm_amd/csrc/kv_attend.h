@@ -189,9 +189,11 @@ struct Ops<true, NP, NS> {
     // pieces of y / most, |y| <= most, for 4 values: piece NP - 1 the lowest
     __device__ __forceinline__ static void pieces(const float *y, float most, uint32_t (&o)[NP]) {
         uint32_t x[4], c[4];
+        const int ex = exponent_of(most);
+        const float to = most > 0.0f ? kQ / __builtin_amdgcn_ldexpf(most, -ex) : 0.0f;
 #pragma unroll
         for (int i = 0; i < 4; i++)
-            x[i] = (uint32_t)(int32_t)__builtin_rintf(most > 0.0f ? y[i] / most * kQ : 0.0f);
+            x[i] = (uint32_t)(int32_t)__builtin_rintf(__builtin_amdgcn_ldexpf(y[i], -ex) * to);
         o[NP - 1] = bytes4<0>(x);
 #pragma unroll
         for (int i = 0; i < 4; i++) c[i] = x[i] + 128u;

@@ -1,11 +1,12 @@
 // The attention of prompts over a paged cache; its instances are in
 // kern_kv_prompt_*.hip, its launches in kern_kv_attn.hip.
 //
-// A block of W waves takes 32 W query rows of one K/V head ((token, query head
-// of the group) pairs), a wave 32 of them, and goes over the context in steps
-// of 64 tokens.  All waves share a step's keys and values, which the block
-// brings into LDS as f16 while it computes the step before (8-bit codes are
-// f16 values: the conversion is done once for 32 W rows).  A step of a wave is
+// A block takes 32 WR query rows of one K/V head ((token, query head of the
+// group) pairs), a wave 32 of them, and goes over the context in steps of 64
+// tokens.  All waves share a step's keys and values, which the block brings into
+// LDS while it computes the step before.  8-bit codes are f16 values: values,
+// and keys but for f16 activations, become f16 on the way, once for all rows.
+// A step of a wave is
 //   S^T = K Q^T     [32 tokens x 32 rows] twice,
 //   p = 2^(S - m),
 //   O^T += V^T P^T  [32 dims x 32 rows] per 32 dims,
@@ -17,6 +18,14 @@
 // two; p enters as one, or as two where activations are f32.  An f16 is as
 // exact for a large p as for a small one, so m need not be the maximum: it is
 // raised, and the sums rescaled, only when some p would pass 2^14 from 2^6.
+// 8-bit pages and f16 activations: two f16 products would be S^T; two integer
+// products (32x32x32, twice the rate) of q's two signed 8-bit pieces with the
+// codes themselves take half of that and half of the LDS (8000 tokens, 32 heads
+// of 128: 632 us against 758; 701 tokens behind 6001, three times: 240 against
+// 276).  For bf16 one f16 product is as fast, and needs no conversion of sums
+// (612 against 634, 226 against 238); for f32 it would be three integer products
+// and sums for each (919 against 942, 350 against 346, and 500 tokens of 16
+// heads 25.9 against 18.4).
 // 8-bit pages: the keys' scale is part of a score's factor.  The values' is
 // part of p's exponent, relative to U, the largest of the steps so far:
 // p' = 2^(S - m + 6 + log2(scale / U)), and l adds p' U / scale.
@@ -27,6 +36,7 @@
 namespace lcmoe {
 
 typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef int32_t intx16 __attribute__((ext_vector_type(16)));
 
 // four codes to four f16: codes + 128 in the last bits of 1024 + (codes + 128)
 __device__ __forceinline__ half4 codes4(uint32_t w) {
@@ -58,6 +68,8 @@ template <int WT> constexpr int kPromptLeast = 2 * WT;
 // m of a row that has met no key
 constexpr float kNone = -1e30f;
 template <int ACT> constexpr int kQPieces = ACT == LCMOE_TYPE_BF16 ? 1 : 2;
+// whether the keys' codes enter as they are
+template <int ACT, bool I8> constexpr bool kCodes = I8 && ACT == LCMOE_TYPE_F16;
 template <int ACT> constexpr int kPPieces = ACT == LCMOE_TYPE_F32 ? 2 : 1;
 
 // What a load has brought, copied here: the compiler would copy it to the next
@@ -75,7 +87,7 @@ __device__ __forceinline__ T arrived(T x) {
 // dims.  Values (r: dim): token groups g and g + 2, of 4 (wide) or 2 (narrow)
 // dims 16 apart.  A wave's items are known by its number alone, and every one
 // is the same two loads, so that nothing waits for a load but its store.
-template <bool I8, int NS, int W>
+template <bool I8, bool CODES, int NS, int W>
 struct Staged {
     static constexpr int NJ = I8 ? NS / 2 : 0, NB = I8 ? NS & 1 : NS;  // wide, narrow blocks
     // items: of each block two of keys, then two of values
@@ -116,26 +128,32 @@ struct Staged {
         }
     }
 
-    // sk [2 tiles of 32 tokens][2 NS sets of 16 dims][2][32 tokens][8 dims]
-    // sv [4 units][NS][2][32 dims][8 tokens]; there: whether the lane's page is.
-    // f16, where `edge` asks: a value that is not finite is stored as zero, and
-    // its token's bit set in bad[dim]; returns whether there is one.
-    __device__ __forceinline__ bool store(half8 *sk, half8 *sv, int wave, int lane, int tokens,
+    // sk [2 tiles of 32 tokens][sets of 32 (codes) or 16 (f16) dims][2][32
+    // tokens][16 bytes]; sv [4 units][NS][2][32 dims][8 tokens]; there: whether
+    // the lane's page is.  f16, where `edge` asks: a value that is not finite is
+    // stored as zero, and its token's bit set in bad[dim]; returns whether there
+    // is one.
+    __device__ __forceinline__ bool store(uintx4 *sk, half8 *sv, int wave, int lane, int tokens,
                                           bool there, bool edge, unsigned long long *bad) const {
         bool odd = false;
         const int unit = lane >> 4, r = lane & 15;
-        half8 *kd = sk + (unit >> 1) * (2 * NS) * 64 + (unit & 1) * 16 + r;
+        uintx4 *kd = sk + (unit >> 1) * (CODES ? NS : 2 * NS) * 64 + (unit & 1) * 16 + r;
         half8 *vd = sv + unit * NS * 64 + r;
 #pragma unroll
         for (int k = 0; k < PW; k++) {
             const int i = wave + k * W, j = i >= 2 * NJ ? i - 2 * NJ : i;
-            if (i < 2 * NJ) {  // dims 64 (j / 2) + 32 (j % 2): sets 2 j, 2 j + 1
+            if (i < 2 * NJ) {  // dims 64 (j / 2) + 32 (j % 2), 16 in each of x
 #pragma unroll
-                for (int c = 0; c < 2; c++)
+                for (int c = 0; c < 2; c++) {
+                    if constexpr (CODES) {
+                        kd[j * 64 + c * 32] = x[k][c];
+                    } else {
 #pragma unroll
-                    for (int g = 0; g < 2; g++)
-                        kd[(2 * j + c) * 64 + g * 32] =
-                            cat(codes4(x[k][c][2 * g]), codes4(x[k][c][2 * g + 1]));
+                        for (int g = 0; g < 2; g++)
+                            kd[(2 * j + c) * 64 + g * 32] = __builtin_bit_cast(
+                                uintx4, cat(codes4(x[k][c][2 * g]), codes4(x[k][c][2 * g + 1])));
+                    }
+                }
             } else if (i < WI) {
 #pragma unroll
                 for (int t = 0; t < 4; t++)
@@ -147,6 +165,10 @@ struct Staged {
         for (int k = 0; k < PN; k++) {
             const int i = wave + k * W;
             if (i >= NI) break;
+            if (CODES && i < 2 * NB) {
+                kd[2 * NJ * 64 + i * 32] = y[k][0];
+                continue;
+            }
             half4 c[4];  // chunk 0, chunk 1: of 8 dims, or of 2 dims by 4 tokens
 #pragma unroll
             for (int t = 0; t < 4; t++)
@@ -154,8 +176,8 @@ struct Staged {
                           : __builtin_bit_cast(half4, uintx2{y[k][t >> 1][2 * (t & 1)],
                                                              y[k][t >> 1][2 * (t & 1) + 1]});
             if (i < 2 * NB) {
-                kd[(4 * NJ + i) * 64] = cat(c[0], c[1]);
-                kd[(4 * NJ + i) * 64 + 32] = cat(c[2], c[3]);
+                kd[(4 * NJ + i) * 64] = __builtin_bit_cast(uintx4, cat(c[0], c[1]));
+                kd[(4 * NJ + i) * 64 + 32] = __builtin_bit_cast(uintx4, cat(c[2], c[3]));
             } else {
                 const int j = i - 2 * NB, g = j & 1, b = 2 * NJ + (j >> 1);
                 if constexpr (!I8) {
@@ -217,7 +239,8 @@ __device__ __forceinline__ void read_ahead() {
 // WT = 1: two buffers, so that a step is brought in beside the one before.
 template <int ACT, bool I8, int NS, int WR, int WT>
 __global__ __launch_bounds__(64 * WR * WT, NS <= 4 ? 2 : 1) void k_attend_prompt(KvArgs a, AttendArgs t) {
-    constexpr int NQ = kQPieces<ACT>, NP = kPPieces<ACT>, KS = 2 * NS, M = 32 * WR;
+    constexpr bool CODES = kCodes<ACT, I8>;
+    constexpr int NQ = kQPieces<ACT>, NP = kPPieces<ACT>, KS = CODES ? NS : 2 * NS, M = 32 * WR;
     constexpr int KB = 2 * KS * 64, VB = 4 * NS * 64, BUFS = WT == 1 ? 2 : WT;
     constexpr int QB = WR * NQ * KS * 64;
     __shared__ __attribute__((aligned(16))) half8 s_kv[BUFS * (KB + VB) > QB ? BUFS * (KB + VB) : QB];
@@ -226,7 +249,8 @@ __global__ __launch_bounds__(64 * WR * WT, NS <= 4 ? 2 : 1) void k_attend_prompt
     // whose values are not finite, by dim; by turn, and whether there are any
     __shared__ unsigned long long s_bad[I8 ? 1 : WT * 4][I8 ? 1 : 32 * NS];
     __shared__ int s_odd[WT][4];
-    half8 *const s_k = s_kv, *const s_v = s_kv + BUFS * KB;
+    uintx4 *const s_k = reinterpret_cast<uintx4 *>(s_kv);
+    half8 *const s_v = s_kv + BUFS * KB;
     const int lane = threadIdx.x & 63, row = lane & 31, g = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wr = wave % WR, wt = wave / WR;
@@ -244,7 +268,7 @@ __global__ __launch_bounds__(64 * WR * WT, NS <= 4 ? 2 : 1) void k_attend_prompt
         return table[min(step * 4 + (lane >> 4), last_unit) >> ushift];
     };
     const auto is_there = [&](int p) { return p >= 0 && p < a.n_pages; };
-    Staged<I8, NS, WR> st;
+    Staged<I8, CODES, NS, WR> st;
     float sks = 0.0f, svs = 0.0f;  // scales of the lane's unit, of the step being brought in
     int page = page_of(step0);
     const auto bring = [&](int step) {
@@ -270,22 +294,34 @@ __global__ __launch_bounds__(64 * WR * WT, NS <= 4 ? 2 : 1) void k_attend_prompt
         for (int k = threadIdx.x; k < WT * 4 * 32 * NS; k += 64 * WR * WT) (&s_bad[0][0])[k] = 0;
         if (threadIdx.x < 4 * WT) (&s_odd[0][0])[threadIdx.x] = 0;
     }
-    // its operands, through LDS: [group of rows][piece][16 dims][lane]
-    half8 *const s_q = s_kv;
+    // its operands, through LDS: [group of rows][piece][set of dims][lane]
+    uintx4 *const s_q = s_k;
     stage_q<NS, M, 64 * WR * WT>(a, t, x, h,
         [&](int64_t e, float (&y)[8]) { load_n<ACT>(t.q, e, y); },
         [&](int r, int c, const float (&y)[8], float most) {
-            half8 o[NQ];
-            half_pieces<NQ>(y, exponent_of(most), o);
+            if constexpr (CODES) {
+                uint32_t o0[NQ], o1[NQ];
+                Ops<true, NQ, NS>::pieces(&y[0], most, o0);
+                Ops<true, NQ, NS>::pieces(&y[4], most, o1);
 #pragma unroll
-            for (int p = 0; p < NQ; p++)
-                s_q[(((r >> 5) * NQ + p) * KS + (c >> 1)) * 64 + (c & 1) * 32 + (r & 31)] = o[p];
+                for (int p = 0; p < NQ; p++)
+                    reinterpret_cast<uintx2 *>(
+                        s_q + (((r >> 5) * NQ + p) * KS + (c >> 2)) * 64 + (c >> 1 & 1) * 32 + (r & 31))[c & 1] =
+                        uintx2{o0[p], o1[p]};
+            } else {
+                half8 o[NQ];
+                half_pieces<NQ>(y, exponent_of(most), o);
+#pragma unroll
+                for (int p = 0; p < NQ; p++)
+                    s_q[(((r >> 5) * NQ + p) * KS + (c >> 1)) * 64 + (c & 1) * 32 + (r & 31)] =
+                        __builtin_bit_cast(uintx4, o[p]);
+            }
         },
         [&](int r, float most, float bad) {
-            s_mul[r] = __builtin_amdgcn_ldexpf(t.scale, exponent_of(most) - 15) * kLog2e + bad;
+            s_mul[r] = Ops<CODES, NQ, NS>::factor(most, t.scale) + bad;
         });
     __syncthreads();
-    half8 qf[NQ][KS];
+    uintx4 qf[NQ][KS];
 #pragma unroll
     for (int p = 0; p < NQ; p++)
 #pragma unroll
@@ -356,23 +392,47 @@ __global__ __launch_bounds__(64 * WR * WT, NS <= 4 ? 2 : 1) void k_attend_prompt
         }
         if (step < step1 && step * 64 < n_tok) {
             const bool whole = !missing && (step + 1) * 64 <= all_see;
-            const half8 *const kp = s_k + buf * KB + lane, *const vp = s_v + buf * VB + lane;
+            const uintx4 *const kp = s_k + buf * KB + lane;
+            const half8 *const vp = s_v + buf * VB + lane;
             floatx16 c[2];
-#pragma unroll
-            for (int tt = 0; tt < 2; tt++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) c[tt][e] = 0.0f;
             // a product on the same sums waits for the one before: turn by turn
+            if constexpr (CODES) {
 #pragma unroll
-            for (int s = 0; s < KS; s++) {
-                half8 ka[2];
+                for (int tt = 0; tt < 2; tt++) {
+                    intx16 n[NQ];
 #pragma unroll
-                for (int tt = 0; tt < 2; tt++) ka[tt] = kp[(tt * KS + s) * 64];
+                    for (int p = 0; p < NQ; p++)
 #pragma unroll
-                for (int p = 0; p < NQ; p++)
+                        for (int e = 0; e < 16; e++) n[p][e] = 0;
 #pragma unroll
-                    for (int tt = 0; tt < 2; tt++)
-                        c[tt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka[tt], qf[p][s], c[tt], 0, 0, 0);
+                    for (int s = 0; s < KS; s++) {
+                        const intx4 ka = __builtin_bit_cast(intx4, kp[(tt * KS + s) * 64]);
+#pragma unroll
+                        for (int p = 0; p < NQ; p++)
+                            n[p] = __builtin_amdgcn_mfma_i32_32x32x32_i8(
+                                ka, __builtin_bit_cast(intx4, qf[p][s]), n[p], 0, 0, 0);
+                    }
+                    // at most 127 (127 256) 256 < 2^31
+#pragma unroll
+                    for (int e = 0; e < 16; e++) c[tt][e] = (float)(n[0][e] * 256 + n[1][e]);
+                }
+            } else {
+#pragma unroll
+                for (int tt = 0; tt < 2; tt++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) c[tt][e] = 0.0f;
+#pragma unroll
+                for (int s = 0; s < KS; s++) {
+                    half8 ka[2];
+#pragma unroll
+                    for (int tt = 0; tt < 2; tt++) ka[tt] = __builtin_bit_cast(half8, kp[(tt * KS + s) * 64]);
+#pragma unroll
+                    for (int p = 0; p < NQ; p++)
+#pragma unroll
+                        for (int tt = 0; tt < 2; tt++)
+                            c[tt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
+                                ka[tt], __builtin_bit_cast(half8, qf[p][s]), c[tt], 0, 0, 0);
+                }
             }
             read_ahead<2 * KS, NQ>();
             // exponents' factors and offsets by unit; l's weights
