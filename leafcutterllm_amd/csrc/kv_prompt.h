@@ -243,6 +243,12 @@ __global__ __launch_bounds__(64 * WR * WT, NS <= 4 ? 2 : 1) void k_attend_prompt
     constexpr int NQ = kQPieces<ACT>, NP = kPPieces<ACT>, KS = CODES ? NS : 2 * NS, M = 32 * WR;
     constexpr int KB = 2 * KS * 64, VB = 4 * NS * 64, BUFS = WT == 1 ? 2 : WT;
     constexpr int QB = WR * NQ * KS * 64;
+    // f16 pages, q's second piece: it stays in LDS, which has the bandwidth to
+    // read it again each step, where registers would not hold it: heads of 96
+    // and 128 dims (8000 tokens of 32 heads of 128: 859 us against 1179, f32
+    // activations 1098 against 1381).  Smaller heads have the registers, larger
+    // ones have not the LDS.
+    constexpr bool LOW = !I8 && NQ == 2 && WT == 1 && (NS == 3 || NS == 4);
     __shared__ __attribute__((aligned(16))) half8 s_kv[BUFS * (KB + VB) > QB ? BUFS * (KB + VB) : QB];
     __shared__ float s_mul[M];
     // f16 pages: of a step that not every row of the block sees, the tokens
@@ -328,6 +334,12 @@ __global__ __launch_bounds__(64 * WR * WT, NS <= 4 ? 2 : 1) void k_attend_prompt
         for (int c = 0; c < KS; c++) qf[p][c] = s_q[((wr * NQ + p) * KS + c) * 64 + lane];
     const float mul = s_mul[32 * wr + row];
     __syncthreads();  // the buffers are the steps' from here on
+    uintx4 *const s_low = s_k + BUFS * (KB + VB) + wr * KS * 64 + lane;
+    if constexpr (LOW) {
+        static_assert(BUFS * (KB + VB) + WR * KS * 64 <= sizeof(s_kv) / 16, "q's pieces took as much");
+#pragma unroll
+        for (int c = 0; c < KS; c++) s_low[c * 64] = qf[1][c];
+    }
 
     floatx16 acc[NS];
 #pragma unroll
@@ -426,6 +438,7 @@ __global__ __launch_bounds__(64 * WR * WT, NS <= 4 ? 2 : 1) void k_attend_prompt
                     half8 ka[2];
 #pragma unroll
                     for (int tt = 0; tt < 2; tt++) ka[tt] = __builtin_bit_cast(half8, kp[(tt * KS + s) * 64]);
+                    if constexpr (LOW) qf[1][s] = s_low[s * 64];
 #pragma unroll
                     for (int p = 0; p < NQ; p++)
 #pragma unroll
@@ -434,7 +447,7 @@ __global__ __launch_bounds__(64 * WR * WT, NS <= 4 ? 2 : 1) void k_attend_prompt
                                 ka[tt], __builtin_bit_cast(half8, qf[p][s]), c[tt], 0, 0, 0);
                 }
             }
-            read_ahead<2 * KS, NQ>();
+            read_ahead<(LOW ? 3 : 2) * KS, LOW ? 1 : NQ>();
             // exponents' factors and offsets by unit; l's weights
             float f[4], off[4], weight[4];
             if constexpr (I8) {
