@@ -241,20 +241,24 @@ template <int ACT, bool I8, int NS, int WR, int WT>
 __global__ __launch_bounds__(64 * WR * WT, NS <= 4 ? 2 : 1) void k_attend_prompt(KvArgs a, AttendArgs t) {
     constexpr bool CODES = kCodes<ACT, I8>;
     constexpr int NQ = kQPieces<ACT>, NP = kPPieces<ACT>, KS = CODES ? NS : 2 * NS, M = 32 * WR;
-    constexpr int KB = 2 * KS * 64, VB = 4 * NS * 64, BUFS = WT == 1 ? 2 : WT;
-    constexpr int QB = WR * NQ * KS * 64;
-    // f16 pages, q's second piece: it stays in LDS, which has the bandwidth to
-    // read it again each step, where registers would not hold it: heads of 96
-    // and 128 dims (8000 tokens of 32 heads of 128: 859 us against 1179, f32
-    // activations 1098 against 1381).  Smaller heads have the registers, larger
-    // ones have not the LDS.
-    constexpr bool LOW = !I8 && NQ == 2 && WT == 1 && (NS == 3 || NS == 4);
-    __shared__ __attribute__((aligned(16))) half8 s_kv[BUFS * (KB + VB) > QB ? BUFS * (KB + VB) : QB];
+    // f16 pages, q's last piece: where registers would not hold it, it stays in
+    // LDS, which has the bandwidth to read it again each step.  Heads of 128 (and
+    // 96) dims: 8000 tokens of 32 heads 854 us against 1156, bf16 activations 676
+    // against 716, 500 tokens of 16 heads 18.3 against 23.0.  Past 192 dims, in
+    // the room of the second buffer: 4000 tokens of 16 heads of 256 279 us against
+    // 934.  Smaller heads have the registers; blocks of 64 rows of larger ones
+    // have not the LDS.
+    constexpr bool LOW = !I8 && (WT == 1 ? NS == 3 || NS == 4 || NS == 8 : NS == 4);
+    constexpr bool TWICE = WT == 1 && !(LOW && NS == 8);
+    constexpr int SLOTS = TWICE ? 4 : 2;
+    constexpr int KB = 2 * KS * 64, VB = 4 * NS * 64, BUFS = TWICE ? 2 : WT;
+    constexpr int QB = WR * NQ * KS * 64, LB = LOW ? WR * KS * 64 : 0, SB = BUFS * (KB + VB) + LB;
+    __shared__ __attribute__((aligned(16))) half8 s_kv[SB > QB ? SB : QB];
     __shared__ float s_mul[M];
     // f16 pages: of a step that not every row of the block sees, the tokens
     // whose values are not finite, by dim; by turn, and whether there are any
-    __shared__ unsigned long long s_bad[I8 ? 1 : WT * 4][I8 ? 1 : 32 * NS];
-    __shared__ int s_odd[WT][4];
+    __shared__ unsigned long long s_bad[I8 ? 1 : WT * SLOTS][I8 ? 1 : 32 * NS];
+    __shared__ int s_odd[WT][SLOTS];
     uintx4 *const s_k = reinterpret_cast<uintx4 *>(s_kv);
     half8 *const s_v = s_kv + BUFS * KB;
     const int lane = threadIdx.x & 63, row = lane & 31, g = lane >> 5;
@@ -297,8 +301,8 @@ __global__ __launch_bounds__(64 * WR * WT, NS <= 4 ? 2 : 1) void k_attend_prompt
     const int n_tok = first < x.rows ? x.s.len0 + min(first + 31, x.rows - 1) / G + 1 : 0;
     if constexpr (!I8) {
 #pragma unroll 1
-        for (int k = threadIdx.x; k < WT * 4 * 32 * NS; k += 64 * WR * WT) (&s_bad[0][0])[k] = 0;
-        if (threadIdx.x < 4 * WT) (&s_odd[0][0])[threadIdx.x] = 0;
+        for (int k = threadIdx.x; k < WT * SLOTS * 32 * NS; k += 64 * WR * WT) (&s_bad[0][0])[k] = 0;
+        if (threadIdx.x < SLOTS * WT) (&s_odd[0][0])[threadIdx.x] = 0;
     }
     // its operands, through LDS: [group of rows][piece][set of dims][lane]
     uintx4 *const s_q = s_k;
@@ -335,11 +339,9 @@ __global__ __launch_bounds__(64 * WR * WT, NS <= 4 ? 2 : 1) void k_attend_prompt
     const float mul = s_mul[32 * wr + row];
     __syncthreads();  // the buffers are the steps' from here on
     uintx4 *const s_low = s_k + BUFS * (KB + VB) + wr * KS * 64 + lane;
-    if constexpr (LOW) {
-        static_assert(BUFS * (KB + VB) + WR * KS * 64 <= sizeof(s_kv) / 16, "q's pieces took as much");
+    if (LOW && wt == 0)
 #pragma unroll
-        for (int c = 0; c < KS; c++) s_low[c * 64] = qf[1][c];
-    }
+        for (int c = 0; c < KS; c++) s_low[c * 64] = qf[NQ - 1][c];
 
     floatx16 acc[NS];
 #pragma unroll
@@ -353,16 +355,18 @@ __global__ __launch_bounds__(64 * WR * WT, NS <= 4 ? 2 : 1) void k_attend_prompt
     // whether some row of the block does not see all of a step
     const auto edge_of = [&](int step) { return (step + 1) * 64 > x.all_see; };
     const auto store = [&](int step, int n, int buf) {
-        unsigned long long *const bad = s_bad[I8 ? 0 : wt * 4 + (n & 3)];
+        unsigned long long *const bad = s_bad[I8 ? 0 : wt * SLOTS + n % SLOTS];
         const bool odd = st.store(s_k + buf * KB, s_v + buf * VB, wr, lane, x.n_tok - step * 64,
                                   is_there(page), edge_of(step), bad);
         if constexpr (!I8) {
-            if (odd) s_odd[wt][n & 3] = 1;
-            // the turn after the next: its last reader passed a barrier ago
-            if (edge_of(step + 2 * WT)) {
-                if (wr == 0 && lane == 0) s_odd[wt][(n + 2) & 3] = 0;
+            if (odd) s_odd[wt][n % SLOTS] = 1;
+            // of the next turn, or with two buffers the one after: its last
+            // reader passed a barrier ago
+            constexpr int AHEAD = SLOTS / 2;
+            if (edge_of(step + AHEAD * WT)) {
+                if (wr == 0 && lane == 0) s_odd[wt][(n + AHEAD) % SLOTS] = 0;
                 for (int k = wr * 64 + lane; k < 32 * NS; k += 64 * WR)
-                    s_bad[wt * 4 + ((n + 2) & 3)][k] = 0;
+                    s_bad[wt * SLOTS + (n + AHEAD) % SLOTS][k] = 0;
             }
         }
     };
@@ -378,14 +382,14 @@ __global__ __launch_bounds__(64 * WR * WT, NS <= 4 ? 2 : 1) void k_attend_prompt
         bring(step);
         page_ahead = page_of(step + WT);
     };
-    if constexpr (WT == 1) {
+    if constexpr (TWICE) {
         store(step0, 0, 0);
         __syncthreads();
         send(step0 + 1);
     }
     for (int n = 0; n < turns; n++) {
-        const int step = step0 + n * WT, buf = WT == 1 ? n & 1 : wt;
-        if constexpr (WT > 1) {
+        const int step = step0 + n * WT, buf = TWICE ? n & 1 : wt;
+        if constexpr (!TWICE) {
             store(step, n, buf);
             __syncthreads();
             send(step + WT);
@@ -438,7 +442,7 @@ __global__ __launch_bounds__(64 * WR * WT, NS <= 4 ? 2 : 1) void k_attend_prompt
                     half8 ka[2];
 #pragma unroll
                     for (int tt = 0; tt < 2; tt++) ka[tt] = __builtin_bit_cast(half8, kp[(tt * KS + s) * 64]);
-                    if constexpr (LOW) qf[1][s] = s_low[s * 64];
+                    if constexpr (LOW) qf[NQ - 1][s] = s_low[s * 64];
 #pragma unroll
                     for (int p = 0; p < NQ; p++)
 #pragma unroll
@@ -553,7 +557,7 @@ __global__ __launch_bounds__(64 * WR * WT, NS <= 4 ? 2 : 1) void k_attend_prompt
             }
             read_ahead<4 * NS, NP>();
             if constexpr (!I8) {
-                if (s_odd[wt][n & 3]) {
+                if (s_odd[wt][n % SLOTS]) {
                     // the rows that see a token whose value is not finite
                     const int last = min(pos - step * 64, 63);
                     const unsigned long long see = last < 0 ? 0 : ~0ull >> (63 - last);
@@ -561,12 +565,12 @@ __global__ __launch_bounds__(64 * WR * WT, NS <= 4 ? 2 : 1) void k_attend_prompt
                     for (int d = 0; d < NS; d++)
 #pragma unroll
                         for (int e = 0; e < 16; e++)
-                            if (s_bad[wt * 4 + (n & 3)][32 * d + 8 * (e / 4) + 4 * g + e % 4] & see)
+                            if (s_bad[wt * SLOTS + n % SLOTS][32 * d + 8 * (e / 4) + 4 * g + e % 4] & see)
                                 acc[d][e] = NAN;
                 }
             }
         }
-        if constexpr (WT == 1) {
+        if constexpr (TWICE) {
             if (n + 1 < turns) store(step + 1, n + 1, buf ^ 1);
             __syncthreads();
             send(step + 2);
