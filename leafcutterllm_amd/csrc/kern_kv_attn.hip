@@ -21,6 +21,19 @@ int splits_for(const KvArgs &a, int64_t tiles, int want, int st, int least) {
 }
 
 // One launch (n = 1) or two: sequences of up to 16 rows, and those of more.
+//
+// Rows of a block: 256 (128 of heads past 128 dims) where 200 blocks of that at
+// least can run, for 256 CUs, else 64, whose waves share the context.  With 32
+// heads on 8 of 128 dims, 8-bit pages, 64 against 256 rows: 1400 tokens, f16
+// activations (175 blocks) 54 us against 62, bf16 57 and 56; 1600 tokens (200)
+// 67 against 70, bf16 72 and 65; 1600 after 10,000, bf16, 495 against 367; 3000
+// tokens on 16 heads of their own (192) 87 against 113.
+//
+// Blocks of 16 rows share a context until 512 run: 100,000 tokens 42 us, with 256
+// 41, 128 51, 2048 46; 8 sequences of 4096 20, 20, 25, 23; 64 of them 69, 71, 69,
+// 88.  Blocks of 64 rows do until 256 run, where there are up to 128 at all: 64
+// tokens on 30,000 68 us, with 512 77, 128 107, unshared 335; 300 on 10,000 (152
+// blocks) 123 unshared, 154 shared.
 int plans(const KvArgs &a, Plan (&p)[2]) {
     const int G = a.H / a.KVH;
     const int64_t most = (int64_t)a.max_new * G;  // rows of one sequence
@@ -39,9 +52,9 @@ int plans(const KvArgs &a, Plan (&p)[2]) {
                          : std::min<int64_t>((int64_t)a.n_rows * G / M + a.n_seq, per * a.n_seq);
         };
         int M = a.hdp <= 128 ? 256 : 128;
-        if (tiles(M) * a.KVH < 96) M = 64;
-        p[n] = {(int)tiles(M), 0, alike ? (int)((most + M - 1) / M) : 0, n ? 16 : 0, INT32_MAX, M};
-        p[n].splits = p[n].tiles * a.KVH > 128 ? 1 : splits_for(a, p[n].tiles, 256, 64, M == 64 ? 16 : 4);
+        if (tiles(M) * a.KVH < 200) M = 64;
+        p[n] = {(int)tiles(M), 1, alike ? (int)((most + M - 1) / M) : 0, n ? 16 : 0, INT32_MAX, M};
+        if (M == 64 && p[n].tiles * a.KVH <= 128) p[n].splits = splits_for(a, p[n].tiles, 256, 64, 16);
         n++;
     }
     return n;

@@ -638,7 +638,8 @@ __global__ __launch_bounds__(64 * WR * WT, NS <= 4 ? 2 : 1) void k_attend_prompt
     l = pair_sum(l);
     const int64_t orow = x.s.row0 + i;
     const int head = h * G + r % G;
-    const float inv = x.parts > 1 ? unit : l == 0.0f ? 0.0f : unit / l;
+    const bool part = WT > 1 && x.parts > 1;  // blocks of many rows share none
+    const float inv = part ? unit : l == 0.0f ? 0.0f : unit / l;
     const int64_t at = (orow * a.H + head) * t.splits + split;
     const auto out = [&](auto put) {
 #pragma unroll
@@ -649,11 +650,11 @@ __global__ __launch_bounds__(64 * WR * WT, NS <= 4 ? 2 : 1) void k_attend_prompt
                                                     acc[d][4 * e + 3]} * inv);
     };
     const int64_t to = orow * t.ldo + (int64_t)head * a.hd;
-    if (x.parts > 1)
+    if (part)
         out([&](int dim, floatx4 o) { *reinterpret_cast<floatx4 *>(t.part_o + at * (32 * NS) + dim) = o; });
     else
         out([&](int dim, floatx4 o) { if (dim < a.hd) store4_any(ACT, t.out, to + dim, o); });
-    if (x.parts > 1 && g == 0) {
+    if (part && g == 0) {
         t.part_ml[2 * at] = m;
         t.part_ml[2 * at + 1] = l;
     }
@@ -668,8 +669,7 @@ hipError_t prompt_launch(const KvArgs &a, const AttendArgs &t, int tiles, bool m
         if (many) a.i8 ? go(k_attend_prompt<ACT, true, NS, MANY, 1>, MANY) : go(k_attend_prompt<ACT, false, NS, MANY, 1>, MANY);
         else a.i8 ? go(k_attend_prompt<ACT, true, NS, 2, SHARES>, 2 * SHARES) : go(k_attend_prompt<ACT, false, NS, 2, SHARES>, 2 * SHARES);
     });
-    if (many) return a.hdp <= 128 ? attend_join<64, 256, kPromptLeast<1>>(a, t, tiles, st)
-                                  : attend_join<64, 128, kPromptLeast<1>>(a, t, tiles, st);
+    if (many) return hipGetLastError();
     return a.hdp <= 128 ? attend_join<64, 64, kPromptLeast<kShares<4>>>(a, t, tiles, st)
                         : attend_join<64, 64, kPromptLeast<kShares<8>>>(a, t, tiles, st);
 }
