@@ -588,12 +588,14 @@ lcmoe_status lcmoe_kv_read_dev(const lcmoe_kv_desc *desc, const lcmoe_kv_pool *p
  * (attention_forward's core, attention.rs:56-115), which lcmoe_kv_append_dev
  * has put there.  q and out: rows of n_head * head_dim, not overlapping.
  * rope: as for the append, q is rotated on the way; NULL: q is taken as it
- * is.  Scores, softmax and sums in f32; an f32 q and its probabilities enter
- * the products as two f16 each, f16 and bf16 ones as one.  A row with nothing
- * to attend to (every page missing) is zeros.  workspace: at least
- * lcmoe_kv_attention_workspace's bytes, 16-byte aligned; its contents do not
- * matter, and calls that may overlap in time (two streams, two graphs) need
- * one each.  The workspace depends on desc and on the batch's three counts. */
+ * is.  Softmax and sums in f32.  The rotated q enters the products with 15 bits
+ * of its row's largest at least (22 for f32 activations; for bf16 ones 11 bits
+ * of each value), the probabilities with 11 bits of each or 15 of the largest
+ * (22 for f32).  A row with nothing to attend to (every page missing) is zeros.
+ * workspace: at least lcmoe_kv_attention_workspace's bytes, 16-byte aligned;
+ * its contents do not matter, and calls that may overlap in time (two streams,
+ * two graphs) need one each.  The workspace depends on desc and on the batch's
+ * three counts. */
 lcmoe_status lcmoe_kv_attention_workspace(const lcmoe_kv_desc *desc, const lcmoe_kv_batch *batch,
                                           size_t *bytes);
 lcmoe_status lcmoe_kv_attention_dev(const lcmoe_kv_desc *desc, const lcmoe_kv_pool *pool,
