@@ -606,8 +606,8 @@ lcmoe_status lcmoe_kv_attention_dev(const lcmoe_kv_desc *desc, const lcmoe_kv_po
 
 /* ---- log probabilities ------------------------------------------------ */
 
-/* For each row of logits [n_rows][vocab] (rows ld elements apart; F32, F16 or
- * BF16): given_lp [n_rows][n_given] = log softmax at the token ids given
+/* For each row of logits [n_rows][vocab] (vocab up to 2^30, rows ld elements
+ * apart; F32, F16 or BF16): given_lp [n_rows][n_given] = log softmax at the token ids given
  * [n_rows][n_given] (0 for an id outside [0, vocab): it adds nothing to a
  * sum); entropy [n_rows] in nats (NULL: not wanted); the n_top (at most
  * LCMOE_LOGPROBS_TOP) largest logits' ids and log probabilities, largest

@@ -154,7 +154,7 @@ lcmoe_status check_rope(const float *rope) {
 lcmoe_status check_logprobs(int32_t type, int64_t ld, int32_t rows, int32_t vocab, int32_t n_given,
                             int32_t n_top) {
     if (!act_ok(type)) return fail(LCMOE_ERR_UNSUPPORTED, "type=%d (F32, F16 or BF16)", type);
-    if (rows < 0 || vocab < 1 || ld < vocab || ld > ((int64_t)1 << 40))
+    if (rows < 0 || vocab < 1 || vocab > (1 << 30) || ld < vocab || ld > ((int64_t)1 << 40))
         return fail(LCMOE_ERR_INVALID_ARG, "n_rows=%d vocab=%d ld=%lld", rows, vocab, (long long)ld);
     if (n_given < 0 || n_given > 65536) return fail(LCMOE_ERR_INVALID_ARG, "n_given=%d outside [0, 65536]", n_given);
     if (n_top < 0 || n_top > LCMOE_LOGPROBS_TOP)

@@ -661,34 +661,39 @@ lcmoe_status create(const lcmoe_model_desc *desc, const lcmoe_model_weights *w,
         m->paged = true;
         m->kv = KV;
         const size_t table = (size_t)D.max_batch * KV.max_pages;
-        try {
-            m->pages_h.assign(table, -1);
-            m->held.assign(D.max_batch, 0);
-            m->free_pages.reserve(KV.n_pages);
-        } catch (const std::bad_alloc &) {
-            return bail(fail(LCMOE_ERR_OUT_OF_MEMORY, "host allocation failed"));
-        }
+        const int64_t n_pos = (int64_t)KV.max_pages * KV.page_tokens;
+        // on the device first: what does not fit there is refused here
+        if ((st = alloc_n(m, &m->pages, table)) || (st = alloc_n(m, &m->rope, (size_t)n_pos * hd)))
+            return bail(st);
         for (auto &L : m->layers)
             if ((st = alloc_n(m, reinterpret_cast<uint8_t **>(&L.pool.k), pool_bytes)) ||
                 (st = alloc_n(m, reinterpret_cast<uint8_t **>(&L.pool.v), pool_bytes)) ||
                 (st = alloc_n(m, reinterpret_cast<uint8_t **>(&L.pool.scale), scale_bytes)))
                 return bail(st);
-        // apply_rotary_emb's angles as the unpaged model has them: f32
-        // products (attention.rs:13-34)
-        const int64_t n_pos = (int64_t)KV.max_pages * KV.page_tokens;
-        std::vector<float> table_h;
+        const int64_t part = std::min<int64_t>(n_pos, 4096);
+        std::vector<float> angles;
         try {
-            table_h.resize((size_t)n_pos * hd);
+            m->pages_h.assign(table, -1);
+            m->held.assign(D.max_batch, 0);
+            m->free_pages.reserve(KV.n_pages);
+            angles.resize((size_t)part * hd);
         } catch (const std::bad_alloc &) {
             return bail(fail(LCMOE_ERR_OUT_OF_MEMORY, "host allocation failed"));
         }
-        for (int64_t p = 0; p < n_pos; p++)
-            for (int i = 0; i < hd / 2; i++) {
-                const float a = (float)p * freq[i];
-                table_h[p * hd + 2 * i] = std::cos(a);
-                table_h[p * hd + 2 * i + 1] = std::sin(a);
-            }
-        if ((st = upload(m, &m->rope, table_h.data(), 4 * table_h.size()))) return bail(st);
+        // apply_rotary_emb's angles as the unpaged model has them: f32
+        // products (attention.rs:13-34)
+        for (int64_t p0 = 0; p0 < n_pos; p0 += part) {
+            const int64_t n = std::min(part, n_pos - p0);
+            for (int64_t p = 0; p < n; p++)
+                for (int i = 0; i < hd / 2; i++) {
+                    const float a = (float)(p0 + p) * freq[i];
+                    angles[p * hd + 2 * i] = std::cos(a);
+                    angles[p * hd + 2 * i + 1] = std::sin(a);
+                }
+            if (hipMemcpy(m->rope + p0 * hd, angles.data(), 4 * (size_t)(n * hd),
+                          hipMemcpyHostToDevice) != hipSuccess)
+                return bail(fail(LCMOE_ERR_HIP, "hipMemcpy of the rope table"));
+        }
         // of every step and every prompt: fewer rows may be split further
         for (int n = 1 - D.max_prompt; n <= D.max_batch; n++) {
             const lcmoe_kv_batch b = n > 0 ? lcmoe_kv_batch{n, n, 1, nullptr, nullptr, nullptr}
@@ -697,18 +702,16 @@ lcmoe_status create(const lcmoe_model_desc *desc, const lcmoe_model_weights *w,
             if ((st = lcmoe_kv_attention_workspace(&KV, &b, &bytes))) return bail(st);
             m->kv_ws_bytes = std::max(m->kv_ws_bytes, bytes);
         }
-        if ((st = alloc_n(m, &m->pages, table)) ||
-            (st = alloc_n(m, reinterpret_cast<uint8_t **>(&m->kv_ws), m->kv_ws_bytes)))
-            return bail(st);
+        if ((st = alloc_n(m, reinterpret_cast<uint8_t **>(&m->kv_ws), m->kv_ws_bytes))) return bail(st);
     }
     if ((st = alloc_n(m, &m->kc, cache)) || (st = alloc_n(m, &m->vc, cache)) ||
         (st = alloc_n(m, &m->lens, D.max_batch)) || (st = alloc_n(m, &m->step, 1)) ||
         (st = alloc_n(m, &m->tok, T)) || (st = alloc_n(m, &m->next, D.max_batch)) ||
         (st = alloc_n(m, &m->out_tok, (size_t)D.max_batch * D.max_ctx)) ||
         (st = alloc_n(m, &m->hidden, T * d)) || (st = alloc_n(m, &m->xn, T * d)) ||
-        (st = alloc_n(m, &m->qkv, T * (H + 2 * KVH) * hd)) || (st = alloc_n(m, &m->qr, T * H * hd)) ||
+        (st = alloc_n(m, &m->qkv, T * (H + 2 * KVH) * hd)) || (st = alloc_n(m, &m->qr, kv ? 0 : T * H * hd)) ||
         (st = alloc_n(m, &m->attn, T * H * hd)) ||
-        (st = alloc_n(m, &m->part, attention_part_floats((int)T, H, hd, D.max_ctx))) ||
+        (st = alloc_n(m, &m->part, kv ? 0 : attention_part_floats((int)T, H, hd, D.max_ctx))) ||
         (st = alloc_n(m, &m->logits, (size_t)D.max_batch * V)))
         return bail(st);
     if (any_rpl) {

@@ -176,7 +176,8 @@ def lp(type=L.TYPE_F32, x=FAKE, ld=100, rows=3, vocab=100, given=FAKE, n_given=1
     (dict(ld=99), 1), (dict(n_given=-1), 1), (dict(n_given=65537), 1), (dict(top=-1), 1),
     (dict(top=33), 1), (dict(x=None), 1), (dict(given=None), 1), (dict(glp=None), 1),
     (dict(tid=None), 1), (dict(tlp=None), 1), (dict(x=FAKE + 2), 1), (dict(given=FAKE + 1), 1),
-    (dict(ent=FAKE + 2), 1), (dict(type=L.TYPE_BF16, x=FAKE + 1), 1)])
+    (dict(ent=FAKE + 2), 1), (dict(type=L.TYPE_BF16, x=FAKE + 1), 1),
+    (dict(vocab=2**30 + 1, ld=2**30 + 1), 1), (dict(vocab=2**31 - 1, ld=2**31), 1)])
 def test_logprobs_refusals(kw, status):
     refused(status, lp, **kw)
 
