@@ -20,29 +20,55 @@ __device__ __forceinline__ int pages_touched(const KvArgs &a, const Seq &s) {
 }
 
 // The 8-bit code of y: to nearest, ties to even, infinities at the ends, NaN
-// as 0.  The product is in 64 bits, where the rounding of y * (1 / scale)
-// cannot move a code that the exact quotient has.
-__device__ __forceinline__ int code_of(double y, double inv) {
-    const double q = __builtin_rint(y * inv);
-    return q == q ? (int)fmin(fmax(q, -127.0), 127.0) : 0;
+// as 0 (the conversion saturates, and makes 0 of NaN; written as the
+// instruction, since the language leaves both undefined).  The product is in 64
+// bits, where the rounding of y * (1 / scale) cannot move a code that the exact
+// quotient has.
+__device__ __forceinline__ uint32_t code_of(double y, double inv) {
+    int q;
+    asm("v_cvt_i32_f64 %0, %1" : "=v"(q) : "v"(__builtin_rint(y * inv)));
+    return (uint32_t)min(max(q, -127), 127);
 }
 
-// f(i, y[c + i], y[h + c + i]) for a key's dims c .. c + 7 and h + c .. h + c +
-// 7 (h = head_dim / 2), rotated by (cos, sin) = rope[c .. c + 7]:
+// y rounded once: to f32 and, where that is not exact, to the neighbour whose
+// last bit is odd, so that rounding to f16 sees on which side y is
+__device__ __forceinline__ _Float16 f16_of(double y) {
+    const float f = (float)y;
+    const double r = y - (double)f;
+    uint32_t u = __float_as_uint(f);
+    if ((r > 0.0 || r < 0.0) && !(u & 1)) u += (r > 0.0) == (f > 0.0f) ? 1u : ~0u;
+    return (_Float16)__uint_as_float(u);
+}
+// |y|, 0 where it is not finite
+__device__ __forceinline__ double finite(double y) {
+    return fabs(y) < INFINITY ? fabs(y) : 0.0;
+}
+__device__ __forceinline__ float finite(float y) {
+    return fabsf(y) < INFINITY ? fabsf(y) : 0.0f;
+}
+
+// A key's dims c .. c + 7 and h + c .. h + c + 7 (h = head_dim / 2), rotated by
+// (cos, sin) = cs[c .. c + 7], or as they are:
 //   y[d] = x[d] cos - x[h + d] sin,  y[h + d] = x[d] sin + x[h + d] cos.
 // Products of two f32 are exact in 64 bits.
-template <int ACT, class F>
-__device__ __forceinline__ void rotated8(const void *src, int64_t e, int h, const float *cs, F f) {
-    float x[8], z[8];
+template <int ACT>
+__device__ __forceinline__ void rotated8(const void *src, int64_t e, int h, const float *cs,
+                                         double (&lo)[8], double (&hi)[8]) {
+    float x[8], z[8], t[16];
     load_n<ACT>(src, e, x);
     load_n<ACT>(src, e + h, z);
-    float t[16];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        t[2 * i] = 1.0f;
+        t[2 * i + 1] = 0.0f;
+    }
     if (cs) __builtin_memcpy(t, cs, 64);
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-        const double c = t[2 * i], s = t[2 * i + 1];
-        if (cs) f(i, x[i] * c - z[i] * s, x[i] * s + z[i] * c);
-        else f(i, (double)x[i], (double)z[i]);
+        const double c = t[2 * i], s = t[2 * i + 1], zs = z[i] * s, xs = x[i] * s;
+        // without an angle what is not finite must not meet the zero
+        lo[i] = x[i] * c - (cs ? zs : 0.0);
+        hi[i] = (cs ? xs : 0.0) + z[i] * c;
     }
 }
 
@@ -87,148 +113,159 @@ __global__ __launch_bounds__(256) void k_kv_append(KvArgs a, const void *__restr
     const int64_t base = unit_base(a, page, h, 0);
     _Float16 *p16 = reinterpret_cast<_Float16 *>(value ? a.v : a.k) + base;
     uint8_t *p8 = (value ? a.v : a.k) + base;
-    const int KC = half / 8;  // 8-dim chunks of a key's half
+    const int KC = half / 8, NB = hdp >> 5;  // 8-dim chunks of a key's half, 32-dim blocks
     const int unit0 = slot0 >> 4, units = ((slot0 + n + 15) >> 4) - unit0;
-    // item i of the units' keys: a slot and its chunk, if it is one of the new
-    const auto key_at = [&](int i, int &slot, int &c) {
-        const int u = i / (16 * KC);
-        c = 8 * ((i - u * 16 * KC) >> 4);
-        slot = (unit0 + u) * 16 + (i & 15);
-        return slot >= slot0 && slot < slot0 + n;
-    };
-    const auto key8 = [&](int slot, int c, auto f) {
-        const int t = slot - slot0, rot = (a.rope_abs ? s.len0 : 0) + t0 + t;
-        rotated8<ACT>(src, (int64_t)(row0 + t) * ld + (int64_t)h * hd + c, half,
-                      rope ? rope + ((int64_t)rot * half + c) * 2 : nullptr, f);
-    };
-    double inv = 0.0;
-    if constexpr (I8) {
-        float *sp = a.scale + ((int64_t)page * a.KVH + h) * 2 + value;
-        const float old = slot0 ? *sp : 0.0f;
-        double most = 0.0;
-        const auto larger = [&](double y) {
-            const double m = fabs(y);
-            if (m > most && m < INFINITY) most = m;
-        };
+    // i / KC and i / NB of up to 16 * 16: exact
+    const int by_kc = 65536 / KC + 1, by_nb = 65536 / NB + 1;
+    double most = 0.0, inv = 0.0;
+    // in 8 bits two turns, the first for the scale: one code for both, as a
+    // line of code that is run once costs as much as it takes to fetch it
+#pragma unroll 1
+    for (int turn = I8 ? 0 : 1; turn < 2; turn++) {
         if (!value) {
-            for (int i = tid; i < units * 16 * KC; i += 256) {
-                int slot, c;
-                if (key_at(i, slot, c))
-                    key8(slot, c, [&](int, double lo, double hi) {
-                        larger(lo);
-                        larger(hi);
-                    });
+#pragma unroll 1
+            for (int i = tid >> 4; i < units * KC; i += 16) {
+                const int u = (i * by_kc) >> 16, c = 8 * (i - u * KC);
+                const int slot = (unit0 + u) * 16 + (tid & 15), t = slot - slot0;
+                if (t < 0 || t >= n) continue;
+                const int rot = (a.rope_abs ? s.len0 : 0) + t0 + t;
+                double lo[8], hi[8];
+                rotated8<ACT>(src, (int64_t)(row0 + t) * ld + (int64_t)h * hd + c, half,
+                              rope ? rope + ((int64_t)rot * half + c) * 2 : nullptr, lo, hi);
+                const int64_t at = (int64_t)(slot >> 4) * 16 * hdp;
+                if constexpr (I8) {
+                    if (!turn) {
+#pragma unroll
+                        for (int e = 0; e < 8; e++) most = fmax(most, fmax(finite(lo[e]), finite(hi[e])));
+                        continue;
+                    }
+                    uintx2 wl, wh;
+#pragma unroll
+                    for (int e = 0; e < 8; e += 4) {
+                        uint32_t ql[4], qh[4];
+#pragma unroll
+                        for (int k = 0; k < 4; k++) {
+                            ql[k] = code_of(lo[e + k], inv);
+                            qh[k] = code_of(hi[e + k], inv);
+                        }
+                        wl[e / 4] = bytes4<0>(ql);
+                        wh[e / 4] = bytes4<0>(qh);
+                    }
+                    *reinterpret_cast<uintx2 *>(p8 + at + k_place<true>(hdp, slot & 15, c)) = wl;
+                    *reinterpret_cast<uintx2 *>(p8 + at + k_place<true>(hdp, slot & 15, half + c)) = wh;
+                } else {
+                    half8 wl, wh;
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        wl[e] = f16_of(lo[e]);
+                        wh[e] = f16_of(hi[e]);
+                    }
+                    *reinterpret_cast<half8 *>(p16 + at + k_place<false>(hdp, slot & 15, c)) = wl;
+                    *reinterpret_cast<half8 *>(p16 + at + k_place<false>(hdp, slot & 15, half + c)) = wh;
+                }
             }
         } else {
-            const int C = hd / 8;
-            for (int i = tid; i < n * C; i += 256) {
-                float x[8];
-                load_n<ACT>(src, (int64_t)(row0 + i / C) * ld + (int64_t)h * hd + 8 * (i % C), x);
+            // 16 items for each unit and 32 dims, the padding's zeros among them
+#pragma unroll 1
+            for (int i = tid; i < units * NB * 16; i += 256) {
+                const int u = ((i >> 4) * by_nb) >> 16, p = (i >> 4) - u * NB, g = (i >> 2) & 3, q = i & 3;
+                const int r0 = 16 * (unit0 + u) + 4 * g - slot0;  // the first of the item's 4 tokens
+                if (r0 + 4 <= 0 || r0 >= n) continue;
+                // every load in bounds and of the page's new rows: what a token
+                // that is not new or a dim past the last brings is not kept
+                const int d = 32 * p + 4 * q, d16 = d + 16 < hd ? d + 16 : d;
+                float x[4][2][4];  // token, 16 dims, dim
 #pragma unroll
-                for (int e = 0; e < 8; e++) larger(x[e]);
-            }
-        }
-        __shared__ double s_most[4];
-        most = wave_max(most);
-        if ((tid & 63) == 0) s_most[tid >> 6] = most;
-        __syncthreads();
-        most = fmax(fmax(s_most[0], s_most[1]), fmax(s_most[2], s_most[3]));
-        const float scale = fmaxf(old, (float)(most / 127.0));
-        inv = scale > 0.0f ? 1.0 / (double)scale : 0.0;
-        if (slot0 && scale > old) {
-            // every code of the units that hold old ones; what lies behind
-            // them is written next, or is not read
-            const double ratio = (double)old / (double)scale;
-            const int words = ((slot0 + 15) >> 4) * 2 * hdp;
-            uintx2 *w = reinterpret_cast<uintx2 *>(p8);
-            for (int i = tid; i < words; i += 256) {
-                const uintx2 c = w[i];
-                uintx2 o = {0, 0};
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const int q = (int)__builtin_rint((double)(int8_t)(c[e >> 2] >> 8 * (e & 3)) * ratio);
-                    o[e >> 2] |= (uint32_t)(uint8_t)q << 8 * (e & 3);
+                for (int e = 0; e < 4; e++) {
+                    const int64_t at = (int64_t)(row0 + min(max(r0 + e, 0), n - 1)) * ld + (int64_t)h * hd;
+                    load_n<ACT>(src, at + min(d, hd - 4), x[e][0]);
+                    load_n<ACT>(src, at + min(d16, hd - 4), x[e][1]);
                 }
-                w[i] = o;
-            }
-        }
-        __syncthreads();  // *sp read by every thread, the moved codes written
-        if (tid == 0) *sp = scale;
-    }
-    if (!value) {
-        for (int i = tid; i < units * 16 * KC; i += 256) {
-            int slot, c;
-            if (!key_at(i, slot, c)) continue;
-            const int64_t u = (int64_t)(slot >> 4) * 16 * hdp;
-            if constexpr (I8) {
-                uintx2 wl = {0, 0}, wh = {0, 0};
-                key8(slot, c, [&](int e, double lo, double hi) {
-                    wl[e >> 2] |= (uint32_t)(uint8_t)code_of(lo, inv) << 8 * (e & 3);
-                    wh[e >> 2] |= (uint32_t)(uint8_t)code_of(hi, inv) << 8 * (e & 3);
-                });
-                *reinterpret_cast<uintx2 *>(p8 + u + k_place<true>(hdp, slot & 15, c)) = wl;
-                *reinterpret_cast<uintx2 *>(p8 + u + k_place<true>(hdp, slot & 15, half + c)) = wh;
-            } else {
-                half8 wl, wh;
-                key8(slot, c, [&](int e, double lo, double hi) {
-                    wl[e] = (_Float16)lo;
-                    wh[e] = (_Float16)hi;
-                });
-                *reinterpret_cast<half8 *>(p16 + u + k_place<false>(hdp, slot & 15, c)) = wl;
-                *reinterpret_cast<half8 *>(p16 + u + k_place<false>(hdp, slot & 15, half + c)) = wh;
-            }
-        }
-        // the dims that pad the head to hdp meet zeros of the query: zeros too
-        if (const int pad = hdp - hd)
-            for (int i = tid; i < pad * n; i += 256) {
-                const int slot = slot0 + i / pad;
-                const int64_t at = (int64_t)(slot >> 4) * 16 * hdp +
-                                   k_place<I8>(hdp, slot & 15, hd + i % pad);
-                if constexpr (I8) p8[at] = 0;
-                else p16[at] = (_Float16)0.0f;
-            }
-        return;
-    }
-    // values: 16 items for each unit and 32 dims, the padding's zeros among them
-    const int NB = hdp >> 5;
-    for (int i = tid; i < units * NB * 16; i += 256) {
-        const int u = i / (16 * NB), p = (i - u * 16 * NB) >> 4, g = (i >> 2) & 3, q = i & 3;
-        const int r0 = 16 * (unit0 + u) + 4 * g - slot0;  // the first of the item's 4 tokens
-        if (r0 + 4 <= 0 || r0 >= n) continue;
-        const bool all = r0 >= 0 && r0 + 4 <= n;
-        float x[4][2][4];  // token, 16 dims, dim
+                if (I8 && !turn) {
+                    float m = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 4; e++)
+                    for (int f = 0; f < 32; f++) m = fmaxf(m, finite(x[f >> 3][f >> 2 & 1][f & 3]));
+                    most = fmax(most, (double)m);
+                    continue;
+                }
+                // of tokens that are not new what is there stays
+                using Word = std::conditional_t<I8, uint32_t, uint64_t>;
+                constexpr int BITS = 2 * sizeof(Word);
+                Word keep = 0;
+                if (r0 < 0) keep |= ((Word)1 << BITS * -r0) - 1;
+                if (r0 + 4 > n) keep |= ~(((Word)1 << BITS * (n - r0)) - 1);
+                int apart;
+                const int64_t at = (int64_t)(unit0 + u) * 16 * hdp + v_item<I8>(hdp, p, g, q, apart);
 #pragma unroll
-            for (int t = 0; t < 2; t++) {
-                const int d = 32 * p + 16 * t + 4 * q;
-                if (d < hd && r0 + e >= 0 && r0 + e < n) {
-                    load_n<ACT>(src, (int64_t)(row0 + r0 + e) * ld + (int64_t)h * hd + d, x[e][t]);
-                } else {
+                for (int k = 0; k < 4; k++) {
+                    Word w[2], old[2];
+                    Word *o = reinterpret_cast<Word *>(I8 ? (void *)(a.v + base + at + k * apart)
+                                                          : (void *)(p16 + at + k * apart));
 #pragma unroll
-                    for (int k = 0; k < 4; k++) x[e][t][k] = 0.0f;
+                    for (int t = 0; t < 2; t++) {
+                        if constexpr (I8) {
+                            uint32_t c[4];
+#pragma unroll
+                            for (int e = 0; e < 4; e++) c[e] = code_of(x[e][t][k], inv);
+                            w[t] = bytes4<0>(c);
+                        } else {
+                            half4 c;
+#pragma unroll
+                            for (int e = 0; e < 4; e++) c[e] = (_Float16)x[e][t][k];
+                            w[t] = __builtin_bit_cast(uint64_t, c);
+                        }
+                        if (d + 16 * t >= hd) w[t] = 0;
+                    }
+                    if (keep) {
+                        __builtin_memcpy(old, __builtin_assume_aligned(o, sizeof(old)), sizeof(old));
+                        w[0] = (w[0] & ~keep) | (old[0] & keep);
+                        w[1] = (w[1] & ~keep) | (old[1] & keep);
+                    }
+                    __builtin_memcpy(__builtin_assume_aligned(o, sizeof(w)), w, sizeof(w));
                 }
             }
-        int apart;
-        const int64_t at = (int64_t)(unit0 + u) * 16 * hdp + v_item<I8>(hdp, p, g, q, apart);
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-            using Code = std::conditional_t<I8, uint8_t, _Float16>;
-            Code w[8];
-#pragma unroll
-            for (int f = 0; f < 8; f++) {
-                if constexpr (I8) w[f] = (uint8_t)code_of(x[f & 3][f >> 2][k], inv);
-                else w[f] = (_Float16)x[f & 3][f >> 2][k];
-            }
-            Code *o = reinterpret_cast<Code *>(a.v) + base + at + k * apart;
-            if (all) {
-                __builtin_memcpy(__builtin_assume_aligned(o, 8 * sizeof(Code)), w, 8 * sizeof(Code));
-            } else {
-#pragma unroll
-                for (int f = 0; f < 8; f++)
-                    if (r0 + (f & 3) >= 0 && r0 + (f & 3) < n) o[f] = w[f];
-            }
         }
+        if constexpr (I8) {
+            if (turn) break;
+            __shared__ double s_most[4];
+            float *sp = a.scale + ((int64_t)page * a.KVH + h) * 2 + value;
+            const float old = slot0 ? *sp : 0.0f;
+            most = wave_max(most);
+            if ((tid & 63) == 0) s_most[tid >> 6] = most;
+            __syncthreads();
+            most = fmax(fmax(s_most[0], s_most[1]), fmax(s_most[2], s_most[3]));
+            const float scale = fmaxf(old, (float)(most / 127.0));
+            inv = scale > 0.0f ? 1.0 / (double)scale : 0.0;
+            if (slot0 && scale > old) {
+                // every code of the units that hold old ones; what lies behind
+                // them is written next, or is not read
+                const double ratio = (double)old / (double)scale;
+                const int words = ((slot0 + 15) >> 4) * 2 * hdp;
+                uintx2 *w = reinterpret_cast<uintx2 *>(p8);
+#pragma unroll 1
+                for (int i = tid; i < words; i += 256) {
+                    const uintx2 c = w[i];
+                    uintx2 o = {0, 0};
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const int q = (int)__builtin_rint((double)(int8_t)(c[e >> 2] >> 8 * (e & 3)) * ratio);
+                        o[e >> 2] |= (uint32_t)(uint8_t)q << 8 * (e & 3);
+                    }
+                    w[i] = o;
+                }
+            }
+            __syncthreads();  // *sp read by every thread, the moved codes written
+            if (tid == 0) *sp = scale;
+        }
+    }
+    // the dims that pad a key to hdp meet zeros of the query: zeros too
+    const int pad = value ? 0 : hdp - hd;
+#pragma unroll 1
+    for (int i = tid; i < pad * n; i += 256) {
+        const int slot = slot0 + i / pad;
+        const int64_t at = (int64_t)(slot >> 4) * 16 * hdp + k_place<I8>(hdp, slot & 15, hd + i % pad);
+        if constexpr (I8) p8[at] = 0;
+        else p16[at] = (_Float16)0.0f;
     }
 }
 

@@ -116,15 +116,6 @@ __device__ __forceinline__ void store4_any(int act, void *p, int64_t e, floatx4 
     else store_n<LCMOE_TYPE_BF16>(p, e, o);
 }
 
-// byte `B` of four words, as one word
-template <int B>
-__device__ __forceinline__ uint32_t bytes4(const uint32_t (&x)[4]) {
-    constexpr uint32_t pair = 0x0c0c0000u | (uint32_t)(B + 4) << 8 | B;
-    const uint32_t a = __builtin_amdgcn_perm(x[1], x[0], pair);
-    const uint32_t b = __builtin_amdgcn_perm(x[3], x[2], pair);
-    return __builtin_amdgcn_perm(b, a, 0x05040100u);
-}
-
 constexpr float kLog2e = 1.44269504088896340736f;
 
 // f16 pieces of 8 values of a row whose largest is `most`, which comes to

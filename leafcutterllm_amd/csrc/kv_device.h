@@ -46,6 +46,15 @@ __device__ __forceinline__ int64_t unit_base(const KvArgs &a, int page, int h, i
     return ((((int64_t)page * a.KVH + h) << (a.plog - 4)) + unit) * 16 * a.hdp;
 }
 
+// byte `B` of four words, as one word
+template <int B>
+__device__ __forceinline__ uint32_t bytes4(const uint32_t (&x)[4]) {
+    constexpr uint32_t pair = 0x0c0c0000u | (uint32_t)(B + 4) << 8 | B;
+    const uint32_t a = __builtin_amdgcn_perm(x[1], x[0], pair);
+    const uint32_t b = __builtin_amdgcn_perm(x[3], x[2], pair);
+    return __builtin_amdgcn_perm(b, a, 0x05040100u);
+}
+
 // Sequence b of the batch: its first row, cached tokens and new tokens, held
 // inside the call's rows and the page table whatever the device arrays say
 // (tokens past the table's capacity are dropped).
