@@ -126,9 +126,7 @@ __device__ __forceinline__ void load_n(const void *base, int64_t e, float (&o)[N
 
 // f32 to bf16, to nearest even (NaN stays NaN)
 __device__ __forceinline__ uint32_t to_bf16(float f) {
-    const uint32_t u = __float_as_uint(f);
-    if ((u & 0x7fffffffu) > 0x7f800000u) return (u >> 16) | 0x40u;
-    return (u + 0x7fffu + ((u >> 16) & 1)) >> 16;
+    return __builtin_bit_cast(uint16_t, (__bf16)f);
 }
 template <int ACT>
 __device__ __forceinline__ uint32_t to16(float f) {
