@@ -81,10 +81,10 @@ __device__ __forceinline__ int v_item(int hdp, int p, int g, int q, int &apart) 
     return v_place<I8>(hdp, 4 * g, 32 * p + 4 * q);
 }
 
-// What bounds it: 4 prompts of 2001 tokens, 8 heads of 128, bf16 into 8 bits, 24
-// us, 1.4 TB/s of what it must move: two passes, and 64-bit arithmetic; one
-// token each of 16 sequences 7.6 us, a chain of dependent loads.  7001 tokens of
-// 16 heads, f32 into f16, one pass, 61 us, 2.9 TB/s.
+// What bounds it: 4 prompts of 2001 tokens, 8 heads of 128, bf16 into 8 bits, 22
+// us, 2.2 TB/s of what it must move: two passes and code to be fetched in one
+// round of blocks; one token each of 16 sequences 6.9 us, a chain of dependent
+// loads.  7001 tokens of 16 heads, f32 into f16, one pass, 43 us, 4.0 TB/s.
 //
 // One block: the new tokens of one page, one K/V head, keys (z = 0) or values
 // (z = 1).  In 8 bits the page's scale S' = max(S, max |new| / 127), S = 0
@@ -276,7 +276,7 @@ __device__ __forceinline__ int units_touched(const Seq &s) {
 
 // One block: one unit of 16 tokens, its K/V heads' items in turn, or a share of
 // them where there are few units.  8 bits to bf16, 8176 tokens of 8 heads of 128:
-// 13.7 us, 3.7 TB/s.
+// 11.6 us, 4.3 TB/s.
 template <int ACT, bool I8>
 __global__ __launch_bounds__(256) void k_kv_read(KvArgs a, void *__restrict__ ko, int64_t ldk,
                                                  void *__restrict__ vo, int64_t ldv) {

@@ -190,6 +190,59 @@ def test_many_rows_and_nonfinite_values(bad):
     np.testing.assert_array_equal(got, want)
 
 
+# heads enough that every one has a block of many rows to itself, whatever its
+# size: tiles of 256 or 128 rows that end early, one after another, over contexts
+# of one step and of many
+@pytest.mark.parametrize("kv", ["i8", "f16"])
+@pytest.mark.parametrize("act", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("hd,lens,new", [(32, [0], [17]), (64, [33, 0], [40, 300]), (96, [0], [150]),
+                                         (128, [0, 75], [18, 290]), (160, [5], [140]), (192, [0], [64]),
+                                         (256, [0, 61], [131, 3])])
+def test_many_heads_of_many_rows(kv, act, hd, lens, new):
+    H, rng = 200, np.random.default_rng(hd + len(act))
+    held = [-(-(a + b) // 32) for a, b in zip(lens, new)]
+    rig = Rig(H, H, hd, 32, kv, act, sum(held), max(held))
+    pages = tables(rng, rig.n_pages, rig.max_pages, held)
+    if any(lens):
+        fill(rig, rng, lens, pages)
+    N = sum(new)
+    rig.append(lens, new, pages, normal(rng, N, H, hd), normal(rng, N, H, hd))
+    rig.check_attention(lens, new, pages, normal(rng, N, H, hd, scale=2.0), every=29)
+
+
+@pytest.mark.parametrize("kv", ["i8", "f16"])
+@pytest.mark.parametrize("act", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_many_heads_and_a_missing_page(kv, act, hd):
+    H, rng = 200, np.random.default_rng(hd)
+    rig = Rig(H, H, hd, 16, kv, act, 20, 18)
+    pages = tables(rng, 20, 18, [18])
+    pages[0, [0, 3, 10]] = -1, 20, -5
+    x = normal(rng, 280, H, hd), normal(rng, 280, H, hd)
+    rig.append([0], [280], pages, *x)
+    rig.check_attention([0], [280], pages, normal(rng, 280, H, hd), every=31)
+
+
+@pytest.mark.parametrize("bad", [np.inf, np.nan])
+@pytest.mark.parametrize("act,hd", [("f32", 64), ("f16", 128), ("bf16", 128), ("f16", 256)])
+def test_many_heads_and_nonfinite_values(bad, act, hd):
+    H, rng = 200, np.random.default_rng(hd)
+    rig = Rig(H, H, hd, 16, "f16", act, 20, 18)
+    pages = tables(rng, 20, 18, [18])
+    k, v, q = (normal(rng, 280, H, hd) for _ in range(3))
+    rig.append([0], [280], pages, k, v)
+    clean = rig.attention([0], [280], pages, q)
+    at = ((37, 3, 5), (63, 3, 63), (64, 7, 0), (130, 199, 33), (279, 11, 12))
+    for tok, head, d in at:
+        v[tok, head, d] = bad
+    rig.append([0], [280], pages, k, v)
+    got = rig.attention([0], [280], pages, q)
+    for tok, head, d in at:
+        assert not np.isfinite(got[tok:, head, d]).any()
+        got[tok:, head, d] = clean[tok:, head, d]
+    np.testing.assert_array_equal(got, clean)
+
+
 @pytest.mark.parametrize("kv", ["i8", "f16"])
 @pytest.mark.parametrize("new", [1, 30])
 def test_missing_pages(kv, new):
