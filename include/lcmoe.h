@@ -658,8 +658,8 @@ lcmoe_status lcmoe_debug_route_fallbacks(lcmoe_handle *h, int32_t *count);
 
 /* Testing of the error path only (no counterpart in the reference): the
  * model's n-th internal forward from now on (0-based; one per prefilled
- * sequence, one per decode step or graph capture) fails before enqueueing
- * anything; n < 0 cancels. */
+ * sequence or scored pass, one per decode step or graph capture) fails before
+ * enqueueing anything; n < 0 cancels. */
 lcmoe_status lcmoe_model_debug_fail_forward(lcmoe_model *m, int32_t n);
 
 /* Observation only (no counterpart in the reference): layer `layer`'s MoE

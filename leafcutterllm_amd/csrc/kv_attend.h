@@ -603,7 +603,7 @@ __global__ __launch_bounds__(256) void k_attend(KvArgs a, AttendArgs t) {
 template <int ST, int M, int LEAST>
 __global__ __launch_bounds__(256) void k_attend_join(KvArgs a, AttendArgs t) {
     __shared__ __attribute__((aligned(16))) floatx4 s_o[256];
-    __shared__ float s_f[128], s_l[128];
+    __shared__ float s_f[128];
     const int h = blockIdx.x % a.KVH, G = a.H / a.KVH, tid = threadIdx.x;
     Tile x;
     if (!find_rows<ST, M, LEAST>(a, t, gridDim.x / a.KVH - 1 - blockIdx.x / a.KVH, x)) return;
@@ -612,19 +612,30 @@ __global__ __launch_bounds__(256) void k_attend_join(KvArgs a, AttendArgs t) {
     const int64_t row = x.s.row0 + r / G;
     const int head = h * G + r % G;
     const int64_t at = (row * a.H + head) * t.splits;
-    if (tid < x.parts) {
-        s_f[tid] = t.part_ml[2 * (at + tid)];
-        s_l[tid] = t.part_ml[2 * (at + tid) + 1];
+    // every wave for itself, two of at most 128 parts a lane: their largest
+    // maximum, their factors, and the sum of their sums
+    float mp[2], lp[2];
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const int s = (tid & 63) + 64 * k;
+        mp[k] = s < x.parts ? t.part_ml[2 * (at + s)] : -INFINITY;
+        lp[k] = s < x.parts ? t.part_ml[2 * (at + s) + 1] : 0.0f;
     }
-    __syncthreads();
-    float top = -INFINITY;
-    for (int s = 0; s < x.parts; s++) top = fmaxf(top, s_f[s]);
+    float top = fmaxf(mp[0], mp[1]);
+    const int lanes = min(x.parts, 64);  // that hold any; the first has their sums
+#pragma unroll 1
+    for (int o = 1; o < lanes; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
     const float base = top == -INFINITY ? 0.0f : top;
-    __syncthreads();
-    if (tid < x.parts) {
-        s_f[tid] = __builtin_amdgcn_exp2f(s_f[tid] - base);
-        s_l[tid] *= s_f[tid];
+    float l = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const float f = __builtin_amdgcn_exp2f(mp[k] - base);
+        if (tid < 64) s_f[tid + 64 * k] = f;
+        l = __builtin_fmaf(lp[k], f, l);
     }
+#pragma unroll 1
+    for (int o = 1; o < lanes; o <<= 1) l += __shfl_xor(l, o, 64);
+    l = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(l)));
     __syncthreads();
     const int C = a.hdp / 4, groups = 256 / C, grp = tid / C, d = 4 * (tid % C);
     floatx4 o = {0, 0, 0, 0};
@@ -638,8 +649,6 @@ __global__ __launch_bounds__(256) void k_attend_join(KvArgs a, AttendArgs t) {
     __syncthreads();
     if (grp || d >= a.hd) return;
     for (int k = 1; k < groups; k++) o += s_o[k * C + tid];
-    float l = 0.0f;
-    for (int s = 0; s < x.parts; s++) l += s_l[s];
     store4_any(a.act, t.out, row * t.ldo + (int64_t)head * a.hd + d,
                o * (l == 0.0f ? 0.0f : 1.0f / l));
 }
